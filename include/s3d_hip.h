@@ -245,6 +245,40 @@ typedef struct S3dAttnArgs {
 int s3d_attention_fwd(const S3dAttnArgs* args, int split, s3d_stream_t stream);
 int s3d_attention_bwd(const S3dAttnArgs* args, s3d_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------ head norm + position rotation
+ * Between the qkv product and the attention (no reference counterpart: timm Attention.forward, visualize_attention_map_voxel.py:125-138, has
+ * neither): every query and key head of a token is divided by its root mean square, multiplied by a gain shared by the heads, and rotated by the
+ * token's position; the value heads pass through.
+ *     z = x / sqrt(mean(x^2) + eps) * gain,   (z_a, z_b) -> (z_a cos - z_b sin, z_b cos + z_a sin)
+ * for the pairs (a, b) = (i, i + hd/2), or (2i, 2i + 1) when `interleaved`.  Rows are tokens: [H query heads | Hkv key heads | Hkv value heads],
+ * hd each (hd a multiple of 16 up to 256); s3d_attention_fwd / _bwd take the result where Hkv == H.
+ *   cos_t / sin_t   [T][hd/2] fp32, or both NULL: no rotation.  A pair that no axis uses has cos 1, sin 0.
+ *   pos             [rows] table row of every token, or NULL: row r takes table row (r / st) % T (st = 1: sequences of T tokens one after the
+ *                   other; st = number of sequences: token-major rows).  A position outside [0, T) leaves the token unrotated (class tokens: -1).
+ *   *_lo            optional low planes of split-bf16 tensors; the gains may be NULL (= 1).
+ * out may be qkv itself (same pointers and pitch; the value heads are then not touched).  For a backward pass keep the input qkv.
+ * Backward: dout = gradient of out; dqkv (may be dout itself) = gradient of qkv; dq_gain / dk_gain [hd] are stored, or added to when
+ * `accumulate`; they are also computed when the gains are NULL.  partial = scratch of partial_blocks >= s3d_qk_norm_blocks(..) times 2 * hd
+ * floats.  No atomics: bitwise reproducible. */
+typedef struct S3dQkNormArgs {
+    const uint16_t* qkv_hi; const uint16_t* qkv_lo; long ld;
+    uint16_t* out_hi; uint16_t* out_lo; long ldo;
+    long rows;
+    int H, Hkv, hd;
+    float eps;
+    const float* q_gain; const float* k_gain;
+    const float* cos_t; const float* sin_t; int T;
+    int st; const int* pos;
+    int interleaved;
+    const uint16_t* dout; const uint16_t* dout_lo; long lddo;
+    uint16_t* dqkv; uint16_t* dqkv_lo; long lddq;
+    float* dq_gain; float* dk_gain; int accumulate;
+    float* partial; int partial_blocks;
+} S3dQkNormArgs;
+int s3d_qk_norm_blocks(long rows, int H, int Hkv, int hd);
+int s3d_qk_norm_rope_fwd(const S3dQkNormArgs* args, s3d_stream_t stream);
+int s3d_qk_norm_rope_bwd(const S3dQkNormArgs* args, s3d_stream_t stream);
+
 /* ------------------------------------------------------------------------------------------------ tokenizers
  * VoxelEmbed.forward (embed_layer_3d_modality.py:170-177), VoxelNaiveProjection.forward (:202-209),
  * VoxelEmbed_no_average.forward (:63-70): s3d_voxel_fold gathers the grid into the patch-GEMM operand
@@ -381,6 +415,44 @@ typedef struct S3dAdamFill {
 int s3d_pack_bf16(const float* src, uint16_t* dst, long n, s3d_stream_t stream);
 int s3d_adam_step_wire(float* p, float* g, const uint16_t* g_wire, float* m, float* v, uint16_t* hi, uint16_t* lo, long n,
                        S3dAdamState* state, int zero_grad, s3d_stream_t stream);
+
+/* ---- orthogonalised updates (no reference counterpart; beside optim.Adam / optim.SGD of train_cls_voxel.py:195, train_partseg.py)
+ * Newton-Schulz: X0 = U / max(|U|_F, eps), then `steps` times  A = X X^T,  X <- a X + (b A + c A^2) X  on the smaller side (a tall matrix is
+ * worked transposed): every singular value s becomes a s + b s^3 + c s^5, the singular vectors stay.  A stack item is `count` matrices
+ * [rows][cols] of one shape: matrix i of a tensor at + i * stride, row pitch ld (elements); any sizes, no alignment beyond the element's;
+ * items with a zero size are skipped.  Products are taken on pairs of fp16 planes with fp32 accumulation (fp32-class, csrc/muon.hip).
+ * Non-finite entries make that matrix's result NaN.  Calls are bitwise reproducible.
+ * workspace: device scratch of at least the size the *_workspace_bytes call gives for the SAME items (16-byte aligned; contents are
+ * neither expected nor kept; two calls that may overlap in time need two).  steps 1 .. 32; coefficients under which a singular value in
+ * [0, 1] would grow past 64 are refused; eps >= 1e-30. */
+typedef struct S3dNsArgs {
+    int steps; float a, b, c; float eps;
+    int x_bf16, out_bf16;             /* s3d_orthogonalize: type of x / out, 1 = bf16, 0 = fp32 */
+    int nesterov, zero_grad;          /* s3d_muon_step */
+} S3dNsArgs;
+typedef struct S3dOrthoItem {
+    const void* x; long x_stride, x_ld;
+    void* out; long out_stride, out_ld;              /* may be x itself (same type, strides and pitch) */
+    int count, rows, cols;
+} S3dOrthoItem;
+size_t s3d_orthogonalize_workspace_bytes(const S3dOrthoItem* items, int n, const S3dNsArgs* args);
+int s3d_orthogonalize(const S3dOrthoItem* items, int n, const S3dNsArgs* args, void* workspace, size_t workspace_bytes, s3d_stream_t stream);
+/* optimizer.step() with orthogonalised momentum for matrix parameters:
+ *     g' = g * grad_scale,  m = mu m + (1 - mu) g',  u = nesterov ? (1 - mu) g' + mu m : m,
+ *     p = p (1 - lr * decay) - lr * scale * NewtonSchulz(u)
+ * hyper (device, 4 floats): {lr, mu, decay, grad_scale} -- in device memory so that a captured step follows a schedule.  hi / lo (both or
+ * none; strides and pitch of p): split-bf16 planes of p, refreshed.  zero_grad != 0 clears g. */
+typedef struct S3dMuonItem {
+    float* p; long p_stride, p_ld;
+    float* g; long g_stride, g_ld;
+    float* m; long m_stride, m_ld;
+    uint16_t* hi; uint16_t* lo;
+    int count, rows, cols;
+    float scale;
+} S3dMuonItem;
+size_t s3d_muon_workspace_bytes(const S3dMuonItem* items, int n, const S3dNsArgs* args);
+int s3d_muon_step(const S3dMuonItem* items, int n, const S3dNsArgs* args, const float* hyper, void* workspace, size_t workspace_bytes,
+                  s3d_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------ mid-graph events for data parallelism
  * DDP (train_cls_voxel.py:155-159, :287) all-reduces gradient buckets while backward is still running.  With HIP graphs that used to

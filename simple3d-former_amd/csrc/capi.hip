@@ -809,7 +809,8 @@ size_t s3d_sizeof(const char* n) {
     SZ(S3dGemmArgs); SZ(S3dLnArgs); SZ(S3dLnBwdArgs); SZ(S3dAttnArgs); SZ(S3dFoldArgs); SZ(S3dPosGradArgs);
     SZ(S3dHeadArgs); SZ(S3dCeArgs); SZ(S3dHeadLossArgs); SZ(S3dAdamState); SZ(S3dBlockShape); SZ(S3dBlockParams); SZ(S3dBlockGrads);
     SZ(S3dBlockActs); SZ(S3dBlockScratch); SZ(S3dEncShape); SZ(S3dEncParams); SZ(S3dEncGrads); SZ(S3dEncActs); SZ(S3dBnArgs);
-    SZ(S3dGroupProjArgs); SZ(S3dAdamFill); SZ(S3dWgradItem); SZ(S3dRowStats); SZ(S3dLnAuxLayer);
+    SZ(S3dGroupProjArgs); SZ(S3dAdamFill); SZ(S3dWgradItem); SZ(S3dRowStats); SZ(S3dLnAuxLayer); SZ(S3dQkNormArgs); SZ(S3dNsArgs);
+    SZ(S3dOrthoItem); SZ(S3dMuonItem);
 #undef SZ
     return 0;
 }
@@ -990,6 +991,27 @@ int s3d_adam_apply_ranges(float* p, float* g, float* m, float* v, uint16_t* hi, 
     return s3d_launch_adam_ranges(p, g, m, v, hi, lo, ranges, n, state, zero_grad, st(s));
 }
 int s3d_pack_bf16(const float* src, uint16_t* dst, long n, s3d_stream_t s) { return s3d_launch_pack_bf16(src, dst, n, st(s)); }
+
+int s3d_qk_norm_rope_fwd(const S3dQkNormArgs* a, s3d_stream_t s) {
+    S3D_REQUIRE(a != nullptr, "s3d_qk_norm_rope_fwd: null args");
+    return s3d_launch_qk_norm_fwd(*a, st(s));
+}
+int s3d_qk_norm_rope_bwd(const S3dQkNormArgs* a, s3d_stream_t s) {
+    S3D_REQUIRE(a != nullptr, "s3d_qk_norm_rope_bwd: null args");
+    return s3d_launch_qk_norm_bwd(*a, st(s));
+}
+size_t s3d_orthogonalize_workspace_bytes(const S3dOrthoItem* items, int n, const S3dNsArgs* a) {
+    return items != nullptr && a != nullptr && n > 0 ? s3d_ortho_workspace(items, n) : 0;
+}
+int s3d_orthogonalize(const S3dOrthoItem* items, int n, const S3dNsArgs* a, void* workspace, size_t workspace_bytes, s3d_stream_t s) {
+    return s3d_launch_orthogonalize(items, n, a, workspace, workspace_bytes, st(s));
+}
+size_t s3d_muon_workspace_bytes(const S3dMuonItem* items, int n, const S3dNsArgs* a) {
+    return items != nullptr && a != nullptr && n > 0 ? s3d_muon_workspace(items, n) : 0;
+}
+int s3d_muon_step(const S3dMuonItem* items, int n, const S3dNsArgs* a, const float* hyper, void* workspace, size_t workspace_bytes, s3d_stream_t s) {
+    return s3d_launch_muon(items, n, a, hyper, workspace, workspace_bytes, st(s));
+}
 
 // ---- events recorded INSIDE a stream capture as external event-record nodes (see s3d_hip.h)
 int s3d_event_create(void** out) {

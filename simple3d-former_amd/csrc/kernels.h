@@ -84,3 +84,13 @@ int s3d_launch_cls_eval(const float* logits, int ld, const long long* target, lo
 int s3d_launch_partseg_eval(const float* logits, int ld, const long long* target, int B, int N, int num_part, const int* part_range,
                             int* pred, double* shape_iou, int* shape_first, long long* counts, hipStream_t s);
 int s3d_launch_unpack_bits(const unsigned int* bits, float* out, long nwords, hipStream_t s);
+
+// ---- head norm + position rotation (qk_norm.hip) ----
+int s3d_launch_qk_norm_fwd(const S3dQkNormArgs& a, hipStream_t s);
+int s3d_launch_qk_norm_bwd(const S3dQkNormArgs& a, hipStream_t s);
+
+// ---- orthogonalised updates (muon.hip) ----
+size_t s3d_ortho_workspace(const S3dOrthoItem* items, int n);
+size_t s3d_muon_workspace(const S3dMuonItem* items, int n);
+int s3d_launch_orthogonalize(const S3dOrthoItem* items, int n, const S3dNsArgs* a, void* workspace, size_t bytes, hipStream_t s);
+int s3d_launch_muon(const S3dMuonItem* items, int n, const S3dNsArgs* a, const float* hyper, void* workspace, size_t bytes, hipStream_t s);

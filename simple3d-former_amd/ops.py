@@ -119,3 +119,203 @@ def cross_entropy(logits, target, weight=None, grad_scale=1.0):
                dlogits=dl, grad_scale=grad_scale)
     L.check(L.lib().s3d_cross_entropy(ctypes.byref(a), L.current_stream()), 'cross_entropy')
     return loss[0], dl
+
+
+# ---------------------------------------------------------------------------------------------- head norm + position rotation
+def _same_device(who, *tensors):
+    """All tensors on the CURRENT device: the call is enqueued on the current stream of it."""
+    dev = torch.device('cuda', torch.cuda.current_device()) if torch.cuda.is_available() else None
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f'{who}: every tensor must be on the current device ({dev}), got one on {t.device}')
+
+
+def _plane(who, name, t, rows, width):
+    """A [rows, >= width] bf16 plane with unit column stride; returns its row pitch."""
+    if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
+        raise ValueError(f'{who}: {name} must be a bfloat16 [{rows}, {width}] tensor with contiguous rows, got {t.dtype} {tuple(t.shape)} {t.stride()}')
+    return t.stride(0) if rows > 1 else max(t.stride(0), width)
+
+
+def rope_table(coords, hd, base=10000.0):
+    """cos / sin table [T, hd/2] (fp32) for s3d_qk_norm_rope: coords [T] positions or [T, A] coordinates on A axes (a voxel grid: A = 3).  Each
+    axis gets (hd/2) // A pairs with angles x * base^(-j / pairs); pairs left over are not rotated.  Angles are formed in 64 bits, so
+    that far positions keep their phase."""
+    c = torch.as_tensor(coords)
+    if c.dim() not in (1, 2) or hd % 16 or not 16 <= hd <= 256:
+        raise ValueError(f'rope_table: coords [T] or [T, A] and a head dim that is a multiple of 16 up to 256, got {tuple(c.shape)}, {hd}')
+    c = c.to(torch.float64)
+    c = c[:, None] if c.dim() == 1 else c
+    T, A = c.shape
+    half, per = hd // 2, hd // 2 // max(A, 1)
+    if A < 1 or per < 1:
+        raise ValueError(f'rope_table: {A} axes for {half} pairs')
+    freq = float(base) ** (-torch.arange(per, dtype=torch.float64, device=c.device) / per)
+    ang = torch.zeros(T, half, dtype=torch.float64, device=c.device)
+    ang[:, :A * per] = (c[:, :, None] * freq).reshape(T, A * per)
+    return ang.cos().float(), ang.sin().float()
+
+
+def _qk_args(who, qkv_hi, qkv_lo, H, hd, Hkv, q_gain, k_gain, rope, pos, st, eps, interleaved, others):
+    Hkv = H if Hkv is None else Hkv
+    if qkv_hi.dim() != 2:
+        raise ValueError(f'{who}: qkv must be [rows, (H + 2 Hkv) hd], got {tuple(qkv_hi.shape)}')
+    rows, W = qkv_hi.shape[0], (H + 2 * Hkv) * hd
+    cos, sin = rope if rope is not None else (None, None)
+    _same_device(who, qkv_hi, qkv_lo, q_gain, k_gain, cos, sin, pos, *others)
+    ld = _plane(who, 'qkv_hi', qkv_hi, rows, W)
+    if qkv_lo is not None and _plane(who, 'qkv_lo', qkv_lo, rows, W) != ld:
+        raise ValueError(f'{who}: the planes of a pair need the same row pitch')
+    for name, g in (('q_gain', q_gain), ('k_gain', k_gain)):
+        if g is not None and (g.dtype != torch.float32 or tuple(g.shape) != (hd,) or not g.is_contiguous()):
+            raise ValueError(f'{who}: {name} must be a contiguous float32 [{hd}] tensor')
+    T = 0
+    if cos is not None:
+        T = cos.shape[0]
+        for t in (cos, sin):
+            if t.dtype != torch.float32 or tuple(t.shape) != (T, hd // 2) or not t.is_contiguous():
+                raise ValueError(f'{who}: the rotation tables must be contiguous float32 [T, {hd // 2}] tensors')
+    if pos is not None and (pos.dtype != torch.int32 or tuple(pos.shape) != (rows,) or not pos.is_contiguous()):
+        raise ValueError(f'{who}: pos must be a contiguous int32 [{rows}] tensor')
+    a = L.fill(L.S3dQkNormArgs(), qkv_hi=qkv_hi, qkv_lo=qkv_lo, ld=ld, rows=rows, H=H, Hkv=Hkv, hd=hd, eps=eps, q_gain=q_gain, k_gain=k_gain,
+               cos_t=cos, sin_t=sin, T=T, st=st, pos=pos, interleaved=1 if interleaved else 0)
+    return a, rows, W
+
+
+def _pair_out(who, name, out, like_hi, like_lo, rows, W):
+    hi, lo = out if out is not None else (torch.empty_like(like_hi, memory_format=torch.contiguous_format),
+                                          None if like_lo is None else torch.empty_like(like_lo, memory_format=torch.contiguous_format))
+    ld = _plane(who, name, hi, rows, W)
+    if lo is not None and _plane(who, name + ' (low plane)', lo, rows, W) != ld:
+        raise ValueError(f'{who}: the planes of a pair need the same row pitch')
+    return hi, lo, ld
+
+
+def qk_norm_rope_fwd(qkv_hi, qkv_lo, H, hd, *, Hkv=None, q_gain=None, k_gain=None, rope=None, pos=None, st=1, eps=1e-6, interleaved=False, out=None):
+    """Root-mean-square norm of every query / key head (gains [hd] fp32, None = 1) and rotation by the token's position, values copied:
+    s3d_qk_norm_rope_fwd.  qkv planes [rows, (H + 2 Hkv) hd] bf16 (qkv_lo None: plain bf16); rope = (cos, sin) of rope_table or None;
+    pos [rows] int32 table rows (outside the table: not rotated) or None: row r takes (r // st) % T.  out = (hi, lo) to write into, which may
+    be the input planes; -> (out_hi, out_lo)."""
+    who = 'qk_norm_rope_fwd'
+    a, rows, W = _qk_args(who, qkv_hi, qkv_lo, H, hd, Hkv, q_gain, k_gain, rope, pos, st, eps, interleaved, out or ())
+    hi, lo, ld = _pair_out(who, 'out', out, qkv_hi, qkv_lo, rows, W)
+    L.fill(a, out_hi=hi, out_lo=lo, ldo=ld)
+    if rows:
+        L.check(L.lib().s3d_qk_norm_rope_fwd(ctypes.byref(a), L.current_stream()), who)
+    return hi, lo
+
+
+def qk_norm_rope_bwd(dout_hi, dout_lo, qkv_hi, qkv_lo, H, hd, *, Hkv=None, q_gain=None, k_gain=None, rope=None, pos=None, st=1, eps=1e-6,
+                     interleaved=False, out=None, gain_grads=None):
+    """Backward of qk_norm_rope_fwd: dout planes (gradient of its output) and the INPUT qkv planes of the forward -> (dqkv_hi, dqkv_lo, dq_gain,
+    dk_gain).  out = (hi, lo) to write dqkv into (may be the dout planes); gain_grads = (dq, dk) to ADD the gains' gradients to."""
+    who = 'qk_norm_rope_bwd'
+    dq, dk = gain_grads if gain_grads is not None else (None, None)
+    a, rows, W = _qk_args(who, qkv_hi, qkv_lo, H, hd, Hkv, q_gain, k_gain, rope, pos, st, eps, interleaved, (dout_hi, dout_lo, dq, dk) + tuple(out or ()))
+    lddo = _plane(who, 'dout_hi', dout_hi, rows, W)
+    if dout_lo is not None and _plane(who, 'dout_lo', dout_lo, rows, W) != lddo:
+        raise ValueError(f'{who}: the planes of a pair need the same row pitch')
+    hi, lo, ld = _pair_out(who, 'out', out, dout_hi, dout_lo, rows, W)
+    if gain_grads is None:
+        dq, dk = torch.empty(2, hd, dtype=torch.float32, device=qkv_hi.device)
+    for g in (dq, dk):
+        if g.dtype != torch.float32 or tuple(g.shape) != (hd,) or not g.is_contiguous():
+            raise ValueError(f'{who}: the gains\' gradients must be contiguous float32 [{hd}] tensors')
+    lib = L.lib()
+    blocks = lib.s3d_qk_norm_blocks(rows, a.H, a.Hkv, hd)
+    part = torch.empty(max(blocks, 1) * 2 * hd, dtype=torch.float32, device=qkv_hi.device)
+    L.fill(a, dout=dout_hi, dout_lo=dout_lo, lddo=lddo, dqkv=hi, dqkv_lo=lo, lddq=ld, dq_gain=dq, dk_gain=dk, accumulate=0 if gain_grads is None else 1,
+           partial=part, partial_blocks=blocks)
+    if rows:
+        L.check(lib.s3d_qk_norm_rope_bwd(ctypes.byref(a), L.current_stream()), who)
+    elif gain_grads is None:
+        dq.zero_()
+        dk.zero_()
+    return hi, lo, dq, dk
+
+
+# ---------------------------------------------------------------------------------------------- orthogonalised updates
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _matrices(who, name, t, dtypes):
+    """[r, c] or [L, r, c] with contiguous rows -> (count, rows, cols, stride, pitch)"""
+    if t.dim() not in (2, 3) or t.dtype not in dtypes:
+        raise ValueError(f'{who}: {name} must be a [rows, cols] or [count, rows, cols] tensor of {" / ".join(str(d) for d in dtypes)}, got {t.dtype} {tuple(t.shape)}')
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f'{who}: the rows of {name} must be contiguous')
+    n = t.shape[0] if t.dim() == 3 else 1
+    r, c = t.shape[-2:]
+    ld = t.stride(-2) if r > 1 else max(c, 1)
+    return n, r, c, (t.stride(0) if n > 1 else r * ld) if t.dim() == 3 else r * ld, ld
+
+
+def _ns_args(steps, coefficients, eps, **kw):
+    a, b, c = coefficients
+    return L.fill(L.S3dNsArgs(), steps=steps, a=a, b=b, c=c, eps=eps, **kw)
+
+
+def orthogonalize(x, *, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dtype=None, out=None):
+    """Newton-Schulz orthogonalisation of a matrix [r, c] or a stack [L, r, c] (fp32 or bf16): s3d_orthogonalize.  The singular values of
+    x / max(|x|_F, eps) go `steps` times through a s + b s^3 + c s^5, the singular vectors stay.  out_dtype: float32 or bfloat16 (default:
+    x's); out: tensor to write into (may be x)."""
+    who = 'orthogonalize'
+    types = (torch.float32, torch.bfloat16)
+    _same_device(who, x, out)
+    n, r, c, xs, xld = _matrices(who, 'x', x, types)
+    if out is None:
+        out = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+    elif out.shape != x.shape or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError(f'{who}: out must have the shape of x and the requested type')
+    _, _, _, os_, old = _matrices(who, 'out', out, types)
+    it = (L.S3dOrthoItem * 1)(L.fill(L.S3dOrthoItem(), x=x, x_stride=xs, x_ld=xld, out=out, out_stride=os_, out_ld=old, count=n, rows=r, cols=c))
+    a = _ns_args(steps, coefficients, eps, x_bf16=int(x.dtype == torch.bfloat16), out_bf16=int(out.dtype == torch.bfloat16))
+    lib = L.lib()
+    size = lib.s3d_orthogonalize_workspace_bytes(it, 1, ctypes.byref(a))
+    ws = torch.empty(max(size, 16), dtype=torch.uint8, device=x.device)
+    L.check(lib.s3d_orthogonalize(it, 1, ctypes.byref(a), L.ptr(ws), size, L.current_stream()), who)
+    return out
+
+
+def muon_scale(scale, rows, cols):
+    """Factor on the learning rate of a rows x cols update: 'original' sqrt(max(1, rows / cols)); 'match_rms_adamw' 0.2 sqrt(max(rows, cols)) (an
+    update of the root mean square that Adam's has); or a number."""
+    if scale == 'original':
+        return max(1.0, rows / cols) ** 0.5
+    if scale == 'match_rms_adamw':
+        return 0.2 * max(rows, cols) ** 0.5
+    return float(scale)
+
+
+def muon_step(params, grads, momenta, hyper, *, planes=None, nesterov=True, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, scale='original',
+              zero_grad=False):
+    """One optimizer step with orthogonalised momentum over matrix parameters, in place: s3d_muon_step.  params / grads / momenta: lists of fp32
+    [r, c] or [L, r, c] tensors (one entry = one stack of equal matrices); hyper: fp32 device tensor {lr, momentum, decay, grad_scale};
+    planes: list of (hi, lo) bf16 tensors laid out like the parameters, refreshed, or None."""
+    who = 'muon_step'
+    f32 = (torch.float32,)
+    if not len(params) == len(grads) == len(momenta) or (planes is not None and len(planes) != len(params)):
+        raise ValueError(f'{who}: params, grads, momenta (and planes) must have the same length')
+    _same_device(who, hyper, *params, *grads, *momenta, *[t for hl in planes or () for t in hl])
+    if hyper.dtype != torch.float32 or hyper.numel() != 4 or not hyper.is_contiguous():
+        raise ValueError(f'{who}: hyper must be a contiguous float32 tensor of 4 values')
+    items = (L.S3dMuonItem * max(len(params), 1))()
+    for i, (p, g, m) in enumerate(zip(params, grads, momenta)):
+        if p.shape != g.shape or p.shape != m.shape:
+            raise ValueError(f'{who}: parameter {i} {tuple(p.shape)}, its gradient {tuple(g.shape)} and momentum {tuple(m.shape)} differ')
+        n, r, c, ps, pld = _matrices(who, f'params[{i}]', p, f32)
+        _, _, _, gs, gld = _matrices(who, f'grads[{i}]', g, f32)
+        _, _, _, ms, mld = _matrices(who, f'momenta[{i}]', m, f32)
+        hi = lo = None
+        if planes is not None:
+            hi, lo = planes[i]
+            for t in (hi, lo):
+                if t.shape != p.shape or _matrices(who, f'planes[{i}]', t, (torch.bfloat16,))[3:] != (ps, pld):
+                    raise ValueError(f'{who}: the planes of parameter {i} must be laid out like it')
+        L.fill(items[i], p=p, p_stride=ps, p_ld=pld, g=g, g_stride=gs, g_ld=gld, m=m, m_stride=ms, m_ld=mld, hi=hi, lo=lo, count=n, rows=r, cols=c,
+               scale=muon_scale(scale, r, c) if r and c else 0.0)
+    a = _ns_args(steps, coefficients, eps, nesterov=int(bool(nesterov)), zero_grad=int(bool(zero_grad)))
+    lib = L.lib()
+    size = lib.s3d_muon_workspace_bytes(items, len(params), ctypes.byref(a))
+    workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=hyper.device)
+    L.check(lib.s3d_muon_step(items, len(params), ctypes.byref(a), L.ptr(hyper), L.ptr(workspace), size, L.current_stream()), who)
