@@ -41,7 +41,9 @@ def grads(L, r, c, seed=0, dtype=torch.float32):
 
 
 SHAPES = [(1, 1, 1), (2, 1, 7), (2, 9, 1), (3, 5, 3), (1, 16, 16), (1, 64, 64), (2, 65, 64), (1, 63, 130), (2, 130, 63), (1, 192, 192), (2, 192, 576), (2, 576, 192),
-          (1, 387, 1000), (1, 1000, 387), (3, 384, 384), (1, 768, 768), (1, 2, 5000), (1, 1031, 129), (5, 128, 256), (1, 129, 257)]
+          (1, 387, 1000), (1, 1000, 387), (3, 384, 384), (1, 768, 768), (1, 2, 5000), (1, 1031, 129), (5, 128, 256), (1, 129, 257),
+          # enough tiles for the large ones: wide, tall, square, padded
+          (12, 384, 1536), (12, 1536, 384), (2, 1536, 1530), (9, 700, 640), (30, 250, 384)]
 
 
 @pytest.mark.parametrize('L,r,c', SHAPES)
@@ -147,6 +149,18 @@ def test_muon_step_over_mixed_stacks(nesterov, scale):
             continue
         assert torch.equal(gr[i], g0[i])
         check_muon(p0[i], g0[i], m0[i], p[i], m[i], hyper, nesterov, ops.muon_scale(scale, s[-2], s[-1]))
+
+
+def test_muon_step_with_large_tiles():
+    """wide, tall and square stacks of one 384-wide model in one step (128 x 128 tiles)"""
+    shapes = [(6, 1152, 384), (6, 384, 384), (6, 1536, 384), (6, 384, 1536), (1, 380, 1530)]
+    g = torch.Generator(device=DEV).manual_seed(0)
+    p, gr, m = [[torch.randn(*s, generator=g, device=DEV) * k for s in shapes] for k in (0.02, 1e-3, 1e-3)]
+    hyper = torch.tensor([2e-3, 0.95, 0.1, 1.0], device=DEV)
+    p0, m0 = [t.clone() for t in p], [t.clone() for t in m]
+    ops.muon_step(p, gr, m, hyper)
+    for i, s in enumerate(shapes):
+        check_muon(p0[i], gr[i], m0[i], p[i], m[i], hyper, True, ops.muon_scale('original', *s[1:]))
 
 
 def test_muon_many_items_and_bitwise_repeat():
