@@ -17,6 +17,8 @@
 #include <math.h>
 #include <string.h>
 
+#include <type_traits>
+
 #include "kernels.h"
 #include "kmajor.h"
 
@@ -33,12 +35,13 @@ struct NsDims {
     int rp, cp, mp;                   // rows, columns and smaller side padded to the tile
     int tall;                         // rows > cols
     int chunks;                       // partial sums of squares per matrix
-    long ws, wsz;                     // first matrix's planes in the workspace / planes per matrix (in halves)
+    long ws, wsz;                     // first matrix's tensors in the workspace / size of one matrix's (in halves)
     long part;                        // first matrix's partial sums
+    int per; unsigned per_inv;        // this launch: workgroups of a matrix, 2^32 / per
 };
 struct NsTable {
     int n;
-    int tile0[NS_ITEMS + 1];          // first workgroup of every stack in this launch
+    unsigned wgs[NS_ITEMS];           // workgroups of every stack in this launch, 0 behind the last
     NsDims d[NS_ITEMS];
 };
 struct NsPtrs {
@@ -51,21 +54,41 @@ struct NsPtrs {
 enum { SRC_F32 = 0, SRC_BF16 = 1, SRC_MUON = 2 };
 enum { EPI_GRAM = 0, EPI_POLY = 1, EPI_MULT = 2, EPI_OUT_F32 = 3, EPI_OUT_BF16 = 4, EPI_UPDATE = 5 };
 
-// Workgroups go round robin over the eight XCDs, each with an L2 of its own: XCD x takes the x-th eighth of the tile list, so that the
-// tiles of one matrix share an L2.
-__device__ __forceinline__ int xcd_order(int wg, int total) {
-    const int q = total >> 3, r = total & 7, x = wg & 7;
-    return x * q + (x < r ? x : r) + (wg >> 3);
+// Workgroups go round robin over the eight XCDs, each with an L2 of its own: XCD x takes the x-th eighth of every stack's workgroups, so that the
+// tiles of one matrix share an L2 and the XCDs have equal shares of long and short products.  The grid is 8 * sum of ceil(wgs / 8): false for
+// what is over.
+struct NsPlace { int it, mat, tile; };
+__device__ __forceinline__ bool ns_place(const NsTable& t, NsPlace& w) {
+    const unsigned per0 = t.d[0].per, inv0 = t.d[0].per_inv;
+    const unsigned x = blockIdx.x & 7, i = blockIdx.x >> 3;
+    unsigned c = 0, r = 0;
+    int it = -1;
+#pragma unroll
+    for (int k = 0; k < NS_ITEMS; ++k) {                             // (straight line, counts behind the last stack are 0: one load instead of a chain)
+        const unsigned n = t.wgs[k], lo = (x * n) >> 3, size = ((x + 1) * n >> 3) - lo;
+        const bool here = i - c < size;
+        it = here ? k : it;
+        r = here ? lo + (i - c) : r;
+        c += size;
+    }
+    if (it < 0) return false;
+    unsigned per = per0, inv = inv0;
+    if (it) { per = t.d[it].per; inv = t.d[it].per_inv; }
+    unsigned q = (unsigned)(((unsigned long long)r * inv) >> 32);    // r / per, at most two short
+    if (r - q * per >= per) ++q;
+    if (r - q * per >= per) ++q;
+    w.it = it; w.mat = (int)q; w.tile = (int)(r - q * per);
+    return true;
 }
-__device__ __forceinline__ int ns_find(const NsTable& t, int wg) {
-    int i = 0;
-    while (i + 1 < t.n && wg >= t.tile0[i + 1]) ++i;
-    return i;
-}
-// planes of one matrix, in halves from its base: X hi | lo [rp][cp] twice (read one, write the other), A hi | lo [mp][mp], P hi | lo [mp][mp]
+// tensors of one matrix, in halves from its base: X [rp][cp] twice (read one, write the other), A [mp][mp], P [mp][mp], each with room for a pair
 __device__ __forceinline__ long off_x(const NsDims& d, int which) { return 2L * d.rp * d.cp * which; }
 __device__ __forceinline__ long off_a(const NsDims& d) { return 4L * d.rp * d.cp; }
 __device__ __forceinline__ long off_p(const NsDims& d) { return 4L * d.rp * d.cp + 2L * d.mp * d.mp; }
+
+// Planes in memory.  A pair is stored in blocks of 32 columns, [hi 32 | lo 32] = one 128-byte line: a stage of 32 k of a row is ONE line (with two
+// separate planes every line was fetched twice, half of it each time: 12 TB/s of useful L2 traffic instead of 20).  A single plane is plain row
+// major, a stage is then 64 k and again one line per row.
+__device__ __forceinline__ long ns_at(bool pair, long r, int c, int ld) { return pair ? r * 2 * ld + ((c >> 5) << 6) + (c & 31) : r * ld + c; }
 
 __device__ __forceinline__ void split_half(float v, half_t& hi, half_t& lo) {
     hi = (half_t)v;
@@ -108,13 +131,24 @@ __device__ __forceinline__ void load8b(const bf16_t* p, int n, float* v) {
     }
 }
 
+__device__ __forceinline__ void store8b(bf16_t* p, int n, const float* v) {
+    if (n == 8 && ((uintptr_t)p & 15) == 0) {
+        *reinterpret_cast<u32x4*>(p) = u32x4{f2bf2(v[0], v[1]), f2bf2(v[2], v[3]), f2bf2(v[4], v[5]), f2bf2(v[6], v[7])};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = f2bf(v[i]);
+    }
+}
+
 // ---- 1. (momentum and) the sum of squares of every matrix: d.chunks partial sums in 64 bits, added in order by the next kernel ----
 template <int SRC>
 __global__ __launch_bounds__(256) void ns_sumsq_kernel(const NsTable t, const NsPtrs p, const float* __restrict__ hyper, int nesterov,
                                                        double* __restrict__ part) {
-    const int it = ns_find(t, blockIdx.x);
+    NsPlace w;
+    if (!ns_place(t, w)) return;
+    const int it = w.it, mat = w.mat, chunk = w.tile;
     const NsDims& d = t.d[it];
-    const int mat = (blockIdx.x - t.tile0[it]) / d.chunks, chunk = (blockIdx.x - t.tile0[it]) - mat * d.chunks;
     const unsigned upr = (d.cols + 7) / 8, total = upr * d.rows;              // units of 8 columns (at most 2^29)
     const unsigned per = (total + d.chunks - 1) / d.chunks, lo = chunk * per, hi = lo + per < total ? lo + per : total;
     float mu = 0.f, gs = 1.f;
@@ -155,11 +189,11 @@ __global__ __launch_bounds__(256) void ns_sumsq_kernel(const NsTable t, const Ns
 // ---- 2. X0 = U / max(|U|, eps) as planes, padding cleared: 2048 elements of [rp][cp] per workgroup ----
 template <int SRC>
 __global__ __launch_bounds__(256) void ns_load_kernel(const NsTable t, const NsPtrs p, const float* __restrict__ hyper, int nesterov,
-                                                      const double* __restrict__ part, float eps, float sx, half_t* __restrict__ ws) {
-    const int it = ns_find(t, blockIdx.x);
+                                                      const double* __restrict__ part, float eps, float sx, int pair, half_t* __restrict__ ws) {
+    NsPlace w;
+    if (!ns_place(t, w)) return;
+    const int it = w.it, mat = w.mat, blk = w.tile;
     const NsDims& d = t.d[it];
-    const int per = (int)((long)d.rp * d.cp / 2048);
-    const int mat = (blockIdx.x - t.tile0[it]) / per, blk = (blockIdx.x - t.tile0[it]) - mat * per;
     __shared__ double red[256];
     {
         double s = 0.;
@@ -200,253 +234,383 @@ __global__ __launch_bounds__(256) void ns_load_kernel(const NsTable t, const NsP
         h[i] = a;
         l[i] = b;
     }
-    half_t* X = ws + d.ws + mat * d.wsz + (long)r * d.cp + c;
+    half_t* X = ws + d.ws + mat * d.wsz + ns_at(pair, r, c, d.cp);
     *reinterpret_cast<half8*>(X) = h;
-    *reinterpret_cast<half8*>(X + (long)d.rp * d.cp) = l;
+    if (pair) *reinterpret_cast<half8*>(X + 32) = l;
 }
 
 // ---- 3. the products ----
-// One operand of a product: rows of k (KM false: element (i, k) at p + i ld + k) or columns (KM true: at p + k ld + i); the tile starts at i = at.
-struct NsOperand { const half_t* p; long plane; int ld, at; };
+// One operand of a product, i the tile's side: element (i, k) at row i, column k (KM false) or at row k, column i (KM true) of a tensor with ld columns;
+// the tile starts at i = at.
+struct NsOperand { const half_t* p; int ld, at; };
 
-template <int T, bool KM>
-__device__ __forceinline__ half8 ns_frag(const unsigned char* tile, int i16, int lane) {
+// One stage of an operand is T x 128 bytes of LDS: T rows of one line (k-contiguous), or 32 (pairs) / 64 k rows of the tile's columns (k-major).
+// Piece q of it is 1 KB = one DMA instruction of a wave; every lane brings 16 bytes, the slot swizzle is applied here.
+template <int T, int PL, bool KM>
+__device__ __forceinline__ unsigned ns_source(const NsOperand& o, int piece, int lane) {           // byte offset from ns_base (at most 128 rows)
+    if constexpr (KM) {
+        constexpr int W = PL * T, WK = W / 8;                        // halves / 16-byte slots of a row
+        const int r = piece * (64 / WK) + lane / WK, chunk = (lane % WK) ^ kmajor_swz<W>(r);
+        return (unsigned)(r * PL * o.ld + chunk * 8) * 2;
+    } else {
+        const int r = piece * 8 + (lane >> 3), chunk = (lane & 7) ^ dma_swz64(r);
+        return (unsigned)(r * PL * o.ld + chunk * 8) * 2;
+    }
+}
+template <int PL, bool KM>
+__device__ __forceinline__ const half_t* ns_base(const NsOperand& o) { return o.p + (KM ? (long)o.at * PL : (long)o.at * PL * o.ld); }
+template <int PL, bool KM>
+__device__ __forceinline__ long ns_step(const NsOperand& o) { return KM ? 64L * o.ld : 64; }      // halves from stage to stage (32 rows of 2 ld, or 64 rows of ld)
+// one piece: every lane's 16 bytes at base + off land lane-linear at LDS byte address dst (all but off wave-uniform).  The compiler does not count the
+// load: it is retired with a counted wait before anything reads the piece.
+__device__ __forceinline__ void ns_dma(const half_t* base, unsigned off, unsigned dst) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(off), "s"(dst), "s"(base)
+                 : "memory");
+}
+// s_waitcnt vmcnt(vm) [lgkmcnt(0)] as the compiler's own instruction: its count of outstanding LDS reads stays right
+template <int VM, bool LGKM>
+__device__ __forceinline__ void ns_wait() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((VM & 15) | (7 << 4) | ((LGKM ? 0 : 15) << 8) | ((VM >> 4) << 14));
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void ns_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// fragment q of rows / columns i16 .. + 15: q = plane (pairs), or which half of the stage's 64 k (single planes)
+template <int T, int PL, bool KM>
+__device__ __forceinline__ half8 ns_frag(const unsigned char* tile, int q, int i16, int lane) {
     if constexpr (!KM) {
         const int r = i16 + (lane & 15);
-        return *reinterpret_cast<const half8*>(tile + r * 64 + (((lane >> 4) ^ dma_swz32(r)) << 4));
+        return *reinterpret_cast<const half8*>(tile + r * 128 + (((q * 4 + (lane >> 4)) ^ dma_swz64(r)) << 4));
     } else {
         typedef __attribute__((ext_vector_type(4))) short short4v;
         typedef __attribute__((address_space(3))) short4v lds_short4;
+        constexpr int W = PL * T;
         struct { short4v a, b; } u;
-        const unsigned ad = kmajor_addr<T>(tile, i16, (lane >> 4) * 8, lane);
+        const unsigned ad = PL == 2 ? kmajor_addr<W>(tile, (i16 >> 5) * 64 + q * 32 + (i16 & 31), (lane >> 4) * 8, lane)
+                                    : kmajor_addr<W>(tile, i16, q * 32 + (lane >> 4) * 8, lane);
         u.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)ad);
-        u.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)(ad + 4 * T * 2));
+        u.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)(ad + 4 * W * 2));
         return __builtin_bit_cast(half8, u);
     }
 }
+template <int F>
+struct NsFrags { half8 l[2][F], r[2][F]; };
+// the fragments [from, to) of the 4 F of a stage, and the products [from, to) of its 3 F^2 (pairs: hi hi, hi lo, lo hi) or 2 F^2 (the two halves of
+// a single-plane stage): numbered so that they can be dealt out between the other instructions of a stage
+template <int T, int F, int PL, bool LK, bool RK>
+__device__ __forceinline__ void ns_read(NsFrags<F>& f, const unsigned char* st, int wr, int wc, int lane, int from = 0, int to = 4 * F) {
+#pragma unroll
+    for (int e = from; e < to; ++e) {
+        const int q = e / (2 * F), i = (e / 2) % F;
+        if (e & 1) f.r[q][i] = ns_frag<T, PL, RK>(st + T * 128, q, wc + i * 16, lane);
+        else f.l[q][i] = ns_frag<T, PL, LK>(st, q, wr + i * 16, lane);
+    }
+}
+template <int PL, int F>
+constexpr int ns_products() { return (PL == 2 ? 3 : 2) * F * F; }
+template <int F, int PL>
+__device__ __forceinline__ void ns_mfma(const NsFrags<F>& f, f32x4 (&acc)[F][F], int from = 0, int to = ns_products<PL, F>()) {
+#pragma unroll
+    for (int e = from; e < to; ++e) {
+        const int q = e / (F * F), i = e / F % F, j = e % F, ql = PL == 2 ? q == 2 : q, qr = PL == 2 ? q == 1 : q;
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.r[qr][j], f.l[ql][i], acc[i][j], 0, 0, 0);
+    }
+}
 
-// acc = sum over k of L(i, k) R(j, k) for a T x T tile: 256 threads = 2 x 2 waves of T/2 x T/2, 32 k per stage, a ring of RING stages filled by
-// LDS-DMA.  PL planes (2: hi hi + hi lo + lo hi).  acc[i][j][e] = C[wr + 16 i + (lane & 15)][wc + 16 j + 4 (lane >> 4) + e].
+// acc = sum over k of L(i, k) R(j, k) for a T x T tile by 2 x 2 waves of T/2 x T/2: a ring of
+// RING stages filled by LDS-DMA; the fragments of the next stage are read while the matrix cores work on this one (a SIMD has
+// two waves: without that the LDS time of a stage adds to its MFMA time).  PL planes (2: hi hi + hi lo + lo hi; stages of 32 k.  1: stages of
+// 64 k).  K is a multiple of 64.  acc[i][j][e] = C[wr + 16 i + (lane & 15)][wc + 16 j + 4 (lane >> 4) + e].
 template <int T, int RING, int PL, bool LK, bool RK>
 __device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& R, int K, unsigned char* smem, f32x4 (&acc)[T / 32][T / 32]) {
-    constexpr int PLANE = T * 64, STAGE = 2 * PL * PLANE;            // bytes; L hi (lo), R hi (lo)
+    constexpr int STAGE = 2 * T * 128;                               // bytes: L, R
     constexpr int PIECES = STAGE / 1024 / 4;                         // 1 KB DMA pieces per wave and stage
     constexpr int F = T / 32;                                        // 16-row fragments per wave and side
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const bf16_t* src[PIECES];
-    long step[PIECES];                                               // (two values; constant per piece after unrolling)
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    // waves 0, 1 bring L, waves 2, 3 bring R
+    const bool right = wave >= 2;
+    const long step = right ? ns_step<PL, RK>(R) : ns_step<PL, LK>(L);
+    const half_t* src = right ? ns_base<PL, RK>(R) : ns_base<PL, LK>(L);
+    unsigned off[PIECES];
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-        const int q = wave * PIECES + i, plane = q / (T / 16), piece = q % (T / 16);
-        const bool right = plane >= PL;
-        const NsOperand& o = right ? R : L;
-        const bool km = right ? RK : LK;
-        const int wk = T / 8;                                        // 16-byte slots of a k-major row
-        const int r = km ? piece * (64 / wk) + lane / wk : piece * 16 + (lane >> 2);
-        const int chunk = km ? (lane % wk) ^ kmajor_swz<T>(r) : (lane & 3) ^ dma_swz32(r);
-        const half_t* pl = o.p + (plane - (right ? PL : 0)) * o.plane;
-        src[i] = reinterpret_cast<const bf16_t*>(km ? pl + (long)r * o.ld + o.at + chunk * 8 : pl + ((long)o.at + r) * o.ld + chunk * 8);
-        step[i] = km ? 32L * o.ld : 32;
+        const int q = (wave & 1) * PIECES + i;
+        off[i] = right ? ns_source<T, PL, RK>(R, q, lane) : ns_source<T, PL, LK>(L, q, lane);
     }
-    const unsigned lds0 = (unsigned)(uintptr_t)smem + wave * PIECES * 1024;
-    const int KT = K / 32;
-    int slot_in = 0, slot = 0;
-    auto issue = [&]() {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            glds16(src[i], __builtin_amdgcn_readfirstlane(lds0 + slot_in * STAGE + i * 1024));
-            src[i] += step[i];
-        }
-        slot_in = slot_in + 1 == RING ? 0 : slot_in + 1;
-    };
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)smem + wave * PIECES * 1024);
+    const int KT = K / (PL == 2 ? 32 : 64);
+    unsigned slot_in = 0, slot = 0;                                  // in bytes
+    auto advance = [](unsigned& s) { s = s == (RING - 1) * STAGE ? 0 : s + STAGE; };
 #pragma unroll
     for (int i = 0; i < F; ++i)
 #pragma unroll
         for (int j = 0; j < F; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < RING - 1 && k < KT; ++k) issue();
+    for (int k = 0; k < RING && k < KT; ++k) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) ns_dma(src, off[i], lds0 + slot_in + i * 1024);
+        src += step;
+        advance(slot_in);
+    }
     const int wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
-    for (int kt = 0; kt < KT; ++kt) {
-        // stage kt has landed when at most the later stages' pieces are outstanding; the barrier also tells that every wave has read
-        // stage kt - 1, whose slot is refilled next
-        if (kt + RING - 2 < KT) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * PIECES) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (kt + RING - 1 < KT) issue();
-        const unsigned char* st = smem + slot * STAGE;
-        slot = slot + 1 == RING ? 0 : slot + 1;
-        half8 l[PL][F], r[PL][F];
+    // stage 0 has landed when at most the later stages' pieces are outstanding
+    if (RING <= KT) ns_wait<(RING - 1) * PIECES, false>();
+    else ns_wait<0, false>();
+    ns_barrier();
+    NsFrags<F> fa, fb;
+    ns_read<T, F, PL, LK, RK>(fa, smem, wr, wc, lane);
+    auto body = [&](int kt, NsFrags<F>& now, NsFrags<F>& next) {
+        // this wave holds stage kt in registers (lgkmcnt) and its pieces of stage kt + 1 have landed; behind the barrier that is true of every wave:
+        // the slot of stage kt can be refilled, stage kt + 1 can be read (behind the last stage: old data that nobody uses)
+        if (RING == 2 || kt + RING > KT) ns_wait<0, true>();
+        else ns_wait<(RING - 2) * PIECES, true>();
+        ns_barrier();
+        const bool more = kt + RING < KT;
+        advance(slot);
+        // the reads lie under the products (finer interleavings of loads, reads and products measured the same or slower)
+        constexpr int M = ns_products<PL, F>();
 #pragma unroll
-        for (int q = 0; q < PL; ++q)
-#pragma unroll
-            for (int i = 0; i < F; ++i) {
-                l[q][i] = ns_frag<T, LK>(st + q * PLANE, wr + i * 16, lane);
-                r[q][i] = ns_frag<T, RK>(st + (PL + q) * PLANE, wc + i * 16, lane);
-            }
-#pragma unroll
-        for (int i = 0; i < F; ++i)
-#pragma unroll
-            for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r[0][j], l[0][i], acc[i][j], 0, 0, 0);
-        if constexpr (PL == 2) {
-#pragma unroll
-            for (int i = 0; i < F; ++i)
-#pragma unroll
-                for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r[1][j], l[0][i], acc[i][j], 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < F; ++i)
-#pragma unroll
-                for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r[0][j], l[1][i], acc[i][j], 0, 0, 0);
-        }
+        for (int i = 0; i < PIECES; ++i)
+            if (more) ns_dma(src, off[i], lds0 + slot_in + i * 1024);
+        ns_mfma<F, PL>(now, acc, 0, M / 3);
+        ns_read<T, F, PL, LK, RK>(next, smem + slot, wr, wc, lane);
+        ns_mfma<F, PL>(now, acc, M / 3, M);
+        src += step;
+        advance(slot_in);
+    };
+    for (int kt = 0; kt < KT; kt += 2) {
+        body(kt, fa, fb);
+        if (kt + 1 < KT) body(kt + 1, fb, fa);
     }
 }
 
-// f0 .. f2: scale factors of the epilogue; low: the planes written are pairs (0: the next product takes the hi plane only)
-template <int T, int RING, int PL, int EPI>
-__global__ __launch_bounds__(256) void ns_gemm_kernel(const NsTable t, const NsPtrs p, half_t* __restrict__ ws, const float* __restrict__ hyper,
-                                                      int which, float f0, float f1, float f2, int low, int zero_grad) {
+// The same for a 64 x 64 tile with the k range dealt to the four waves (stage s to wave s % 4): every wave works the whole tile on its own
+// stages, brought by itself, so nothing is waited for but its own loads; a quarter of the serial length and half the LDS reads per product.  The
+// four partial sums are added through LDS in the order of the waves.  out[j][e] = C[16 wave + (lane & 15)][16 j + 4 (lane >> 4) + e].
+template <int RING, int PL, bool LK, bool RK>
+__device__ __forceinline__ void ns_product_ksplit(const NsOperand& L, const NsOperand& R, int K, unsigned char* smem, f32x4 (&out)[4]) {
+    constexpr int T = 64, STAGE = 2 * T * 128, PIECES = STAGE / 1024, F = 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    unsigned char* mine = smem + wave * RING * STAGE;
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)mine);
+    const int KT = (K / (PL == 2 ? 32 : 64) - wave + 3) / 4;         // stages wave, wave + 4, ..
+    const long step_l = ns_step<PL, LK>(L), step_r = ns_step<PL, RK>(R);
+    const half_t *src_l = ns_base<PL, LK>(L) + wave * step_l, *src_r = ns_base<PL, RK>(R) + wave * step_r;
+    unsigned off[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) off[i] = i >= PIECES / 2 ? ns_source<T, PL, RK>(R, i - PIECES / 2, lane) : ns_source<T, PL, LK>(L, i, lane);
+    unsigned slot = 0;                                               // in bytes
+    auto issue = [&](unsigned at) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) ns_dma(i >= PIECES / 2 ? src_r : src_l, off[i], lds0 + at + i * 1024);
+        src_l += 4 * step_l;
+        src_r += 4 * step_r;
+    };
+    f32x4 acc[F][F];
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < RING && k < KT; ++k) issue(k * STAGE);
+    for (int kt = 0; kt < KT; ++kt) {
+        if (kt + RING <= KT) ns_wait<(RING - 1) * PIECES, false>();
+        else ns_wait<0, false>();
+        NsFrags<F> f;
+        ns_read<T, F, PL, LK, RK>(f, mine + slot, 0, 0, lane);
+        ns_wait<63, true>();                                         // the slot is in registers: refill it
+        if (kt + RING < KT) issue(slot);
+        slot = slot == (RING - 1) * STAGE ? 0 : slot + STAGE;
+        ns_mfma<F, PL>(f, acc);
+    }
+    // partial sums: 16 KB per wave in its own ring (read by nobody any more), then rows 16 wave .. + 15 from all four
+    f32x4* red = reinterpret_cast<f32x4*>(mine);
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j) red[(i * F + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < F; ++j) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v += reinterpret_cast<const f32x4*>(smem + w * RING * STAGE)[(wave * F + j) * 64 + lane];
+        out[j] = v;
+    }
+}
+
+// How a tile is worked.  TILE_128: 128 x 128, four waves, 66 KB of LDS: two workgroups share a CU, one's start and epilogue lie under the other's
+// products.  TILE_64: 64 x 64, the k range over the four waves: launches with too few 128 x 128 tiles for the CUs.
+enum { TILE_128 = 0, TILE_64 = 1 };
+template <int KIND>
+struct NsTile {
+    static constexpr int T = KIND == TILE_64 ? 64 : 128, PITCH = T + 4;
+    static constexpr int SUM_BYTES = T * PITCH * 4;                  // the tile in fp32
+    static constexpr int RING_BYTES = KIND == TILE_64 ? 4 * 2 * 16384 : 2 * 32768;
+    static constexpr int SUM_AT = KIND == TILE_64 ? RING_BYTES : 0;  // over the ring, except where the ring still holds partial sums
+    static constexpr int BYTES = KIND == TILE_64 ? RING_BYTES + SUM_BYTES : SUM_BYTES > RING_BYTES ? SUM_BYTES : RING_BYTES;
+};
+
+// 8 elements of a tensor of the iteration at column c (a multiple of 8), stored as a pair or as one plane
+__device__ __forceinline__ void ns_store8(half_t* base, bool pair, long r, int c, int ld, const float* v) {
+    half8 h, l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { half_t a, b; split_half(v[e], a, b); h[e] = a; l[e] = b; }
+    half_t* o = base + ns_at(pair, r, c, ld);
+    *reinterpret_cast<half8*>(o) = h;
+    if (pair) *reinterpret_cast<half8*>(o + 32) = l;
+}
+
+// f0 .. f2: scale factors of the epilogue; low: what is written are pairs (0: the next product takes one plane)
+template <int KIND, int PL, int EPI>
+__global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : 2) void ns_gemm_kernel(
+    const NsTable t, const NsPtrs p, half_t* __restrict__ ws, const float* __restrict__ hyper, int which, float f0, float f1, float f2, int low, int zero_grad) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    constexpr int F = T / 32;
+    using Tile = NsTile<KIND>;
+    constexpr int T = Tile::T, PITCH = Tile::PITCH;
     constexpr bool SYM = EPI == EPI_GRAM || EPI == EPI_POLY;
-    const int wg = xcd_order(blockIdx.x, gridDim.x);
-    const int it = ns_find(t, wg);
-    const NsDims& d = t.d[it];
-    const int tm = d.mp / T, tc = d.cp / T;
-    const int per = SYM ? tm * (tm + 1) / 2 : (d.rp / T) * tc;
-    const int mat = (wg - t.tile0[it]) / per, tile = (wg - t.tile0[it]) - mat * per;
+    NsPlace w;
+    if (!ns_place(t, w)) return;
+    const int it = w.it, mat = w.mat, tile = w.tile;
+    NsDims d = t.d[0];                                               // (loaded with the counts; the others cost a second round trip)
+    if (it) d = t.d[it];
     int ti, tj;
     if constexpr (SYM) {                                             // lower triangle, row by row: tile = ti (ti + 1) / 2 + tj
-        ti = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
-        while (ti * (ti + 1) / 2 > tile) --ti;
-        while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
+        ti = __builtin_amdgcn_readfirstlane((int)((__builtin_amdgcn_sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f));
+        if (ti * (ti + 1) / 2 > tile) --ti;
+        if ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
         tj = tile - ti * (ti + 1) / 2;
     } else {
+        const int tc = d.cp / T;
         ti = tile / tc;
         tj = tile - ti * tc;
     }
     half_t* base = ws + d.ws + mat * d.wsz;
-    const long xx = (long)d.rp * d.cp, mm = (long)d.mp * d.mp;
     const half_t* X = base + off_x(d, which);
-    f32x4 acc[F][F];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    float* S = reinterpret_cast<float*>(smem + Tile::SUM_AT);        // the tile, [T][PITCH]
+    auto product = [&](auto lk, auto rk, const NsOperand& L, const NsOperand& R, int K) {
+        constexpr bool LK = decltype(lk)::value, RK = decltype(rk)::value;
+        if constexpr (KIND == TILE_64) {
+            f32x4 acc[4];
+            ns_product_ksplit<2, PL, LK, RK>(L, R, K, smem, acc);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(S + (wave * 16 + (lane & 15)) * PITCH + j * 16 + (lane >> 4) * 4) = acc[j];
+        } else {
+            f32x4 acc[T / 32][T / 32];
+            ns_product<T, 2, PL, LK, RK>(L, R, K, smem, acc);
+            float* mine = S + ((wave >> 1) * (T / 2) + (lane & 15)) * PITCH + (wave & 1) * (T / 2) + (lane >> 4) * 4;
+            __syncthreads();                                         // every wave has read its last stage: the ring is free
+#pragma unroll
+            for (int i = 0; i < T / 32; ++i)
+#pragma unroll
+                for (int j = 0; j < T / 32; ++j) *reinterpret_cast<f32x4*>(mine + i * 16 * PITCH + j * 16) = acc[i][j];
+        }
+        __syncthreads();
+    };
+    const std::false_type rows;                                      // operand stored as rows of k
+    const std::true_type kmajor;
     if constexpr (EPI == EPI_GRAM) {
-        const NsOperand L = {X, xx, d.cp, ti * T}, R = {X, xx, d.cp, tj * T};
-        if (!d.tall) ns_product<T, RING, PL, false, false>(L, R, d.cp, smem, acc);
-        else ns_product<T, RING, PL, true, true>(L, R, d.rp, smem, acc);
+        const NsOperand L = {X, d.cp, ti * T}, R = {X, d.cp, tj * T};
+        if (!d.tall) product(rows, rows, L, R, d.cp);
+        else product(kmajor, kmajor, L, R, d.rp);
     } else if constexpr (EPI == EPI_POLY) {
-        const NsOperand L = {base + off_a(d), mm, d.mp, ti * T}, R = {base + off_a(d), mm, d.mp, tj * T};
-        ns_product<T, RING, PL, false, false>(L, R, d.mp, smem, acc);
+        const NsOperand L = {base + off_a(d), d.mp, ti * T}, R = {base + off_a(d), d.mp, tj * T};
+        product(rows, rows, L, R, d.mp);
     } else {
         const half_t* P = base + off_p(d);
-        if (!d.tall) {
-            const NsOperand L = {P, mm, d.mp, ti * T}, R = {X, xx, d.cp, tj * T};
-            ns_product<T, RING, PL, false, true>(L, R, d.mp, smem, acc);
-        } else {
-            const NsOperand L = {X, xx, d.cp, ti * T}, R = {P, mm, d.mp, tj * T};
-            ns_product<T, RING, PL, false, false>(L, R, d.mp, smem, acc);
-        }
+        if (!d.tall) product(rows, kmajor, NsOperand{P, d.mp, ti * T}, NsOperand{X, d.cp, tj * T}, d.mp);
+        else product(rows, rows, NsOperand{X, d.cp, ti * T}, NsOperand{P, d.mp, tj * T}, d.mp);
     }
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int row = ti * T + (wave >> 1) * (T / 2) + (lane & 15), col = tj * T + (wave & 1) * (T / 2) + (lane >> 4) * 4;
     float lr = 0.f, keep = 1.f;
     if constexpr (EPI == EPI_UPDATE) { lr = hyper[0]; keep = 1.f - lr * hyper[2]; lr *= p.scale[it]; }
+    half_t* O = base + (EPI == EPI_GRAM ? off_a(d) : EPI == EPI_POLY ? off_p(d) : off_x(d, which ^ 1));
+    const int ld = SYM ? d.mp : d.cp;
+    // rows of the tile, 8 columns per thread
+#pragma unroll 4
+    for (int u = tid; u < T * T / 8; u += 256) {
+        const int lrow = u / (T / 8), lcol = (u % (T / 8)) * 8, r = ti * T + lrow, c = tj * T + lcol;
+        float* sp = S + lrow * PITCH + lcol;
+        float v[8];
+        {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(sp), b = *reinterpret_cast<const f32x4*>(sp + 4);
 #pragma unroll
-    for (int i = 0; i < F; ++i)
+            for (int e = 0; e < 4; ++e) { v[e] = a[e] * f0; v[4 + e] = b[e] * f0; }
+        }
+        // GRAM: f0 = sA / sX^2.  POLY: (a I + b A + c A^2) sP: f0 = c sP / sA^2, f1 = b sP / sA, f2 = a sP.  MULT: f0 = sX' / (sP sX).  Last: 1 / (sP sX)
+        if constexpr (EPI == EPI_POLY) {
+            const half_t* A = base + off_a(d) + ns_at(PL == 2, r, c, d.mp);
+            const half8 ah = *reinterpret_cast<const half8*>(A);
+            half8 al = {0, 0, 0, 0, 0, 0, 0, 0};
+            if constexpr (PL == 2) al = *reinterpret_cast<const half8*>(A + 32);
 #pragma unroll
-        for (int j = 0; j < F; ++j) {
-            const int r = row + i * 16, c = col + j * 16;
-            f32x4 v = acc[i][j];
-            if constexpr (SYM || EPI == EPI_MULT) {
-                half_t* O;
-                long ld, pl;
-                if constexpr (EPI == EPI_GRAM) {                     // f0 = sA / sX^2
-                    v *= f0;
-                    O = base + off_a(d); ld = d.mp; pl = mm;
-                } else if constexpr (EPI == EPI_POLY) {              // v = (a I + b A + c A^2) sP: f0 = c sP / sA^2, f1 = b sP / sA, f2 = a sP
-                    const half_t* A = base + off_a(d) + (long)r * d.mp + c;
-                    const half4 ah = *reinterpret_cast<const half4*>(A);
-                    half4 al = {0, 0, 0, 0};
-                    if constexpr (PL == 2) al = *reinterpret_cast<const half4*>(A + mm);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = fmaf(v[e], f0, f1 * ((float)ah[e] + (float)al[e])) + (r == c + e ? f2 : 0.f);
-                    O = base + off_p(d); ld = d.mp; pl = mm;
-                } else {                                             // f0 = sX' / (sP sX)
-                    v *= f0;
-                    O = base + off_x(d, which ^ 1); ld = d.cp; pl = xx;
-                }
-                half4 h, l;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) { half_t a, b; split_half(v[e], a, b); h[e] = a; l[e] = b; }
-                *reinterpret_cast<half4*>(O + (long)r * ld + c) = h;
-                if (low) *reinterpret_cast<half4*>(O + pl + (long)r * ld + c) = l;
-                if (SYM && ti != tj) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) O[(long)(c + e) * ld + r] = h[e];
-                    if (low) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) O[pl + (long)(c + e) * ld + r] = l[e];
-                    }
-                }
-            } else {                                                 // f0 = 1 / (sP sX)
-                if (r >= d.rows || c >= d.cols) continue;
-                v *= f0;
-                const long oi = mat * p.os[it] + (long)r * p.old[it] + c;
-                const int n = d.cols - c < 4 ? d.cols - c : 4;
-                if constexpr (EPI == EPI_OUT_BF16) {
-                    bf16_t* o = (bf16_t*)p.o[it] + oi;
-                    if (n == 4 && ((uintptr_t)o & 7) == 0) *reinterpret_cast<u32x2*>(o) = u32x2{f2bf2(v[0], v[1]), f2bf2(v[2], v[3])};
-                    else
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (e < n) o[e] = f2bf(v[e]);
-                    continue;
-                }
-                float* o = (float*)p.o[it] + oi;
-                const bool vec = n == 4 && ((uintptr_t)o & 15) == 0;
-                if constexpr (EPI == EPI_UPDATE) {
-                    f32x4 w = {0.f, 0.f, 0.f, 0.f};
-                    if (vec) w = *reinterpret_cast<const f32x4*>(o);
-                    else
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (e < n) w[e] = o[e];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = fmaf(-lr, v[e], w[e] * keep);
-                    if (p.hi[it]) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (e < n) {
-                                bf16_t h, l;
-                                split_bf16(v[e], h, l);
-                                p.hi[it][oi + e] = h;
-                                p.lo[it][oi + e] = l;
-                            }
-                    }
-                    if (zero_grad) {
-                        float* g = (float*)p.x[it] + mat * p.xs[it] + (long)r * p.xld[it] + c;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (e < n) g[e] = 0.f;
-                    }
-                }
-                if (vec) *reinterpret_cast<f32x4*>(o) = v;
-                else
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (e < n) o[e] = v[e];
+            for (int e = 0; e < 8; ++e) v[e] = fmaf(f1, (float)ah[e] + (float)al[e], v[e]) + (r == c + e ? f2 : 0.f);
+        }
+        if constexpr (SYM) {
+            if (ti != tj) {                                          // for the mirror image
+                *reinterpret_cast<f32x4*>(sp) = f32x4{v[0], v[1], v[2], v[3]};
+                *reinterpret_cast<f32x4*>(sp + 4) = f32x4{v[4], v[5], v[6], v[7]};
             }
         }
+        if constexpr (SYM || EPI == EPI_MULT) ns_store8(O, low, r, c, ld, v);
+        else {
+            const int n = r < d.rows ? (d.cols - c < 8 ? d.cols - c : 8) : 0;
+            if (n <= 0) continue;
+            const long oi = mat * p.os[it] + (long)r * p.old[it] + c;
+            if constexpr (EPI == EPI_OUT_F32) store8f((float*)p.o[it] + oi, n, v);
+            if constexpr (EPI == EPI_OUT_BF16) store8b((bf16_t*)p.o[it] + oi, n, v);
+            if constexpr (EPI == EPI_UPDATE) {
+                float q[8];
+                load8f((const float*)p.o[it] + oi, n, q);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = fmaf(-lr, v[e], q[e] * keep);
+                store8f((float*)p.o[it] + oi, n, v);
+                if (p.hi[it]) {
+                    store8b(p.hi[it] + oi, n, v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] -= bf2f(f2bf(v[e]));
+                    store8b(p.lo[it] + oi, n, v);
+                }
+                if (zero_grad) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+                    store8f((float*)p.x[it] + mat * p.xs[it] + (long)r * p.xld[it] + c, n, v);
+                }
+            }
+        }
+    }
+    if constexpr (SYM) {
+        if (ti == tj) return;
+        __syncthreads();
+        // the mirror image: 4 x 16 (8 columns of the output) x (rows of the output) per wave: one line per 4 lanes, LDS columns two lanes a bank
+#pragma unroll 2
+        for (int u = tid; u < T * T / 8; u += 256) {
+            const int g = u >> 6, lcol8 = (g % (T / 32)) * 4 + (u & 3), lrow = (g / (T / 32)) * 16 + ((u >> 2) & 15);
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = S[(lcol8 * 8 + e) * PITCH + lrow];
+            ns_store8(O, low, (long)tj * T + lrow, ti * T + lcol8 * 8, ld, v);
+        }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
 struct NsPlan {
     NsTable t;
-    int T;                            // tile
+    int pad;                          // sides are padded to multiples of it: 64 or 128
     long parts;                       // partial sums in front of the planes
     size_t bytes;
 };
 inline int up(int x, int to) { return (x + to - 1) / to * to; }
 
-// Tile of a round by its padded elements: 128 x 128 tiles halve the LDS and L2 traffic of a product, 64 x 64 tiles pad less and spread over more CUs.
-int tile_of(long padded64, long padded128) {
-    return padded128 / (128 * 128) >= 256 && padded128 <= padded64 + padded64 / 4 ? 128 : 64;
-}
+// Padding of a round: multiples of 128 allow the 128 x 128 tiles; not for sides that would grow by much or rounds too small to use them.
+int pad_of(long padded64, long padded128) { return padded128 / (128 * 128) >= 128 && padded128 <= padded64 + padded64 / 4 ? 128 : 64; }
 // the stacks [0, n) of one round: orientation, padding, workspace layout (partial sums first, then the planes)
 bool ns_plan(NsPlan& pl, int n, const int* count, const int* rows, const int* cols) {
     memset(&pl, 0, sizeof(pl));
@@ -454,13 +618,13 @@ bool ns_plan(NsPlan& pl, int n, const int* count, const int* rows, const int* co
     long padded[2] = {0, 0};
     for (int i = 0; i < n; ++i)
         for (int k = 0; k < 2; ++k) padded[k] += (long)count[i] * up(rows[i], 64 << k) * up(cols[i], 64 << k);
-    pl.T = tile_of(padded[0], padded[1]);
+    pl.pad = pad_of(padded[0], padded[1]);
     long off = 0;
     for (int i = 0; i < n; ++i) {
         NsDims& d = pl.t.d[i];
         d.count = count[i]; d.rows = rows[i]; d.cols = cols[i];
         d.tall = rows[i] > cols[i];
-        d.rp = up(rows[i], pl.T); d.cp = up(cols[i], pl.T); d.mp = d.tall ? d.cp : d.rp;
+        d.rp = up(rows[i], pl.pad); d.cp = up(cols[i], pl.pad); d.mp = d.tall ? d.cp : d.rp;
         const long units = ((long)cols[i] + 7) / 8 * rows[i], chunks = (units + 1023) / 1024;
         d.chunks = (int)(chunks > 512 ? 512 : chunks);
         d.part = pl.parts;
@@ -474,19 +638,20 @@ bool ns_plan(NsPlan& pl, int n, const int* count, const int* rows, const int* co
     return true;
 }
 enum { TILES_SUMSQ, TILES_LOAD, TILES_SYM, TILES_MULT };
-// first workgroup of every stack for one kind of launch; the number of workgroups, -1: more than a grid holds
-long ns_tiles(NsTable& t, int T, int kind) {
+// workgroups of every stack for one kind of launch on tiles of T; the size of the grid, -1: more than a grid holds
+long ns_grid(NsTable& t, int T, int kind) {
     long at = 0;
     for (int i = 0; i < t.n; ++i) {
-        t.tile0[i] = (int)at;
-        const NsDims& d = t.d[i];
+        NsDims& d = t.d[i];
         const long tm = d.mp / T;
         const long per = kind == TILES_SUMSQ ? d.chunks : kind == TILES_LOAD ? (long)d.rp * d.cp / 2048 : kind == TILES_SYM ? tm * (tm + 1) / 2 : (long)(d.rp / T) * (d.cp / T);
-        at += per * d.count;
-        if (at > 0x7fffffffL) return -1;
+        if (per * d.count >= (1L << 28)) return -1;
+        d.per = (int)per;
+        d.per_inv = per > 1 ? (unsigned)((1ULL << 32) / per) : 0xffffffffu;
+        t.wgs[i] = (unsigned)(per * d.count);
+        at += (t.wgs[i] + 7) / 8 * 8;
     }
-    t.tile0[t.n] = (int)at;
-    return at;
+    return at < (1L << 31) ? at : -1;
 }
 float pow2_under(double top, double bound) {     // largest power of two s with s * bound <= top
     int e;
@@ -506,25 +671,50 @@ double ns_bounds(double bound, double a, double b, double c, double& pmax) {
     return xmax > 1e-3 ? xmax * 1.01 : 1e-3;
 }
 
-template <int EPI, int T, int RING, int PL>
-int launch_gemm_v(const NsTable& t, const NsPtrs& p, half_t* ws, const float* hyper, int which, float f0, float f1, float f2, int low, int zero_grad,
-                  long tiles, hipStream_t s) {
-    constexpr int bytes = RING * 2 * PL * T * 64;
-    auto k = ns_gemm_kernel<T, RING, PL, EPI>;
-    if (bytes > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(256), bytes, s, t, p, ws, hyper, which, f0, f1, f2, low, zero_grad);
-    S3D_CHECK_LAUNCH_V("newton_schulz", T * 100 + PL * 10 + EPI);
+struct NsScale { float f0, f1, f2; int low, zero_grad; };
+// Which tile a launch takes: the shorter estimate from times measured on pairs of planes, in us.  A 64 x 64 tile has a CU to itself: 5 for its start
+// and end + 0.9 per 128 k.  A 128 x 128 tile: 5 + 0.85 per 32 k alone on its CU, 5 + 1.15 per 32 k for two that share it.  Measured for the whole
+// chain of five steps, 64 / 128 alone (tiles of 128 in the symmetric products / in P X): 12 x 384^2 (72 / 108) 166 / 236 us, 16 x 384^2 (96 / 144)
+// 251 / 239, 4 x 768^2 (84 / 144) 326 / 354, 12 x 768^2 (252 / 432) 657 / 469, 8 x 384 x 1536 (48 / 288) 277 / 374, 16 x (96 / 576) 493 / 439.
+bool tile_128(const NsTable& t, bool gram, bool sym, int planes) {
+    double n64 = 0., w64 = 0., n128 = 0., w128 = 0., longest = 0.;
+    for (int i = 0; i < t.n; ++i) {
+        const NsDims& d = t.d[i];
+        const double k = (gram ? (d.tall ? d.rp : d.cp) : d.mp) * (planes == 2 ? 1. : 0.5);
+        const double m6 = d.mp / 64, m12 = d.mp / 128;
+        const double a = d.count * (sym ? m6 * (m6 + 1) / 2 : (double)(d.rp / 64) * (d.cp / 64));
+        const double b = d.count * (sym ? m12 * (m12 + 1) / 2 : (double)(d.rp / 128) * (d.cp / 128));
+        n64 += a; w64 += a * (5. + 0.9 * k / 128);
+        n128 += b; w128 += b * (5. + 1.15 * k / 32);
+        if (5. + 0.85 * k / 32 > longest) longest = 5. + 0.85 * k / 32;
+    }
+    const double t64 = ceil(n64 / 256) * w64 / n64, t128 = n128 <= 256 ? longest : ceil(n128 / 512) * w128 / n128;
+    return t128 < t64;
+}
+template <int KIND, int PL, int EPI>
+int launch_gemm_v(const NsTable& t, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& f, long grid, hipStream_t s) {
+    using Tile = NsTile<KIND>;
+    auto k = ns_gemm_kernel<KIND, PL, EPI>;
+    if (Tile::BYTES > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, Tile::BYTES);
+    hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(256), Tile::BYTES, s, t, p, ws, hyper, which, f.f0, f.f1, f.f2, f.low, f.zero_grad);
+    S3D_CHECK_LAUNCH_V("newton_schulz", KIND * 100 + PL * 10 + EPI);
     return 0;
 }
 template <int EPI>
-int launch_gemm(int T, int pl, const NsTable& t, const NsPtrs& p, half_t* ws, const float* hyper, int which, float f0, float f1, float f2, int low,
-                int zero_grad, long tiles, hipStream_t s) {
-    if (T == 128) {
-        if (pl == 2) return launch_gemm_v<EPI, 128, 2, 2>(t, p, ws, hyper, which, f0, f1, f2, low, zero_grad, tiles, s);
-        return launch_gemm_v<EPI, 128, 4, 1>(t, p, ws, hyper, which, f0, f1, f2, low, zero_grad, tiles, s);
+int launch_gemm(NsPlan& pl, int planes, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& f, hipStream_t s) {
+    constexpr bool SYM = EPI == EPI_GRAM || EPI == EPI_POLY;
+    const int kind = SYM ? TILES_SYM : TILES_MULT;
+    long grid;
+    if (pl.pad == 128 && tile_128(pl.t, EPI == EPI_GRAM, SYM, planes)) {
+        grid = ns_grid(pl.t, 128, kind);
+        S3D_REQUIRE(grid >= 0, "newton_schulz: too many tiles");
+        if (planes == 2) return launch_gemm_v<TILE_128, 2, EPI>(pl.t, p, ws, hyper, which, f, grid, s);
+        return launch_gemm_v<TILE_128, 1, EPI>(pl.t, p, ws, hyper, which, f, grid, s);
     }
-    if (pl == 2) return launch_gemm_v<EPI, 64, 4, 2>(t, p, ws, hyper, which, f0, f1, f2, low, zero_grad, tiles, s);
-    return launch_gemm_v<EPI, 64, 4, 1>(t, p, ws, hyper, which, f0, f1, f2, low, zero_grad, tiles, s);
+    grid = ns_grid(pl.t, 64, kind);
+    S3D_REQUIRE(grid >= 0, "newton_schulz: too many tiles");
+    if (planes == 2) return launch_gemm_v<TILE_64, 2, EPI>(pl.t, p, ws, hyper, which, f, grid, s);
+    return launch_gemm_v<TILE_64, 1, EPI>(pl.t, p, ws, hyper, which, f, grid, s);
 }
 
 template <int SRC, int LAST>
@@ -532,34 +722,29 @@ int ns_run(NsPlan& pl, const NsPtrs& p, const S3dNsArgs& a, const float* hyper, 
     double* part = reinterpret_cast<double*>(workspace);
     half_t* ws = reinterpret_cast<half_t*>(part + pl.parts);
     NsTable& t = pl.t;
-    long at = ns_tiles(t, pl.T, TILES_SUMSQ);
+    long at = ns_grid(t, 64, TILES_SUMSQ);
     S3D_REQUIRE(at >= 0, "newton_schulz: too many matrices");
     hipLaunchKernelGGL(ns_sumsq_kernel<SRC>, dim3((unsigned)at), dim3(256), 0, s, t, p, hyper, a.nesterov, part);
     S3D_CHECK_LAUNCH_V("newton_schulz_sumsq", SRC);
-    double bound = 1.001;
-    float sx = pow2_under(32768., bound);
-    at = ns_tiles(t, pl.T, TILES_LOAD);
-    S3D_REQUIRE(at >= 0, "newton_schulz: too many tiles");
-    hipLaunchKernelGGL(ns_load_kernel<SRC>, dim3((unsigned)at), dim3(256), 0, s, t, p, hyper, a.nesterov, part, a.eps, sx, ws);
-    S3D_CHECK_LAUNCH_V("newton_schulz_load", SRC);
-    const long sym = ns_tiles(t, pl.T, TILES_SYM);
     // Results kept in bf16: the last two steps run on the hi planes alone.  What they round (2^-12) is multiplied by at most a and 1 before the
     // result, which adds about 1e-3 to the 1.7e-3 (2-norm) of the result's own rounding, whatever the spectrum; a third such step would triple it.
     const int plain_from = LAST == EPI_OUT_BF16 ? a.steps - 2 : a.steps;
+    double bound = 1.001;
+    float sx = pow2_under(32768., bound);
+    at = ns_grid(t, 64, TILES_LOAD);
+    S3D_REQUIRE(at >= 0, "newton_schulz: too many tiles");
+    hipLaunchKernelGGL(ns_load_kernel<SRC>, dim3((unsigned)at), dim3(256), 0, s, t, p, hyper, a.nesterov, part, a.eps, sx, plain_from > 0, ws);
+    S3D_CHECK_LAUNCH_V("newton_schulz_load", SRC);
     for (int k = 0; k < a.steps; ++k) {
         double pmax;
         const double next = ns_bounds(bound, a.a, a.b, a.c, pmax);
         const float sa = pow2_under(32768., bound * bound), sp = pow2_under(32768., pmax), sn = pow2_under(32768., next);
         const int planes = k >= plain_from ? 1 : 2, low = planes == 2, low_x = k + 1 < plain_from;
-        ns_tiles(t, pl.T, TILES_SYM);
-        if (int rc = launch_gemm<EPI_GRAM>(pl.T, planes, t, p, ws, hyper, k & 1, sa / (sx * sx), 0.f, 0.f, low, 0, sym, s)) return rc;
-        if (int rc = launch_gemm<EPI_POLY>(pl.T, planes, t, p, ws, hyper, k & 1, a.c * sp / (sa * sa), a.b * sp / sa, a.a * sp, low, 0, sym, s)) return rc;
-        at = ns_tiles(t, pl.T, TILES_MULT);
-        if (k + 1 < a.steps) {
-            if (int rc = launch_gemm<EPI_MULT>(pl.T, planes, t, p, ws, hyper, k & 1, sn / (sp * sx), 0.f, 0.f, low_x, 0, at, s)) return rc;
-        } else {
-            if (int rc = launch_gemm<LAST>(pl.T, planes, t, p, ws, hyper, k & 1, 1.f / (sp * sx), 0.f, 0.f, 0, a.zero_grad, at, s)) return rc;
-        }
+        if (int rc = launch_gemm<EPI_GRAM>(pl, planes, p, ws, hyper, k & 1, {sa / (sx * sx), 0.f, 0.f, low, 0}, s)) return rc;
+        if (int rc = launch_gemm<EPI_POLY>(pl, planes, p, ws, hyper, k & 1, {a.c * sp / (sa * sa), a.b * sp / sa, a.a * sp, low, 0}, s)) return rc;
+        const int rc = k + 1 < a.steps ? launch_gemm<EPI_MULT>(pl, planes, p, ws, hyper, k & 1, {sn / (sp * sx), 0.f, 0.f, low_x, 0}, s)
+                                       : launch_gemm<LAST>(pl, planes, p, ws, hyper, k & 1, {1.f / (sp * sx), 0.f, 0.f, 0, a.zero_grad}, s);
+        if (rc) return rc;
         sx = sn;
         bound = next;
     }
@@ -583,24 +768,44 @@ int ns_check_shape(const char* who, int i, int count, int rows, int cols) {
     S3D_REQUIRE(rows <= 65536 && cols <= 65536 && count <= (1 << 20), "%s: item %d is too large (%d x %d x %d)", who, i, count, rows, cols);
     return 0;
 }
-template <typename Item>
-size_t ns_workspace(const Item* items, int n) {
-    size_t most = 0;
-    int count[NS_ITEMS], rows[NS_ITEMS], cols[NS_ITEMS], k = 0;
-    NsPlan pl;
+// The non-empty items in rounds of up to NS_ITEMS stacks, the longest products first (the workgroups that start last are then short ones):
+// run(indices, number, rows, cols, count) until it returns non-zero.
+template <typename Item, typename Run>
+int ns_rounds(const Item* items, int n, Run run) {
+    int idx[NS_ITEMS], k = 0;
     for (int i = 0; i <= n; ++i) {
         if (k == NS_ITEMS || (i == n && k > 0)) {
+            NsPlan pl;
+            int count[NS_ITEMS], rows[NS_ITEMS], cols[NS_ITEMS];
+            for (int j = 0; j < k; ++j) { count[j] = items[idx[j]].count; rows[j] = items[idx[j]].rows; cols[j] = items[idx[j]].cols; }
             ns_plan(pl, k, count, rows, cols);
-            if (pl.bytes > most) most = pl.bytes;
+            if (int rc = run(pl, idx, k)) return rc;
             k = 0;
         }
         if (i == n) break;
-        if (ns_check_shape("newton_schulz", i, items[i].count, items[i].rows, items[i].cols)) return 0;
-        if (items[i].count == 0 || items[i].rows == 0 || items[i].cols == 0) continue;
-        count[k] = items[i].count; rows[k] = items[i].rows; cols[k] = items[i].cols;
-        ++k;
+        const Item& q = items[i];
+        if (q.count == 0 || q.rows == 0 || q.cols == 0) continue;
+        const int len = q.rows > q.cols ? q.rows : q.cols;
+        int at = k++;
+        for (; at > 0; --at) {
+            const Item& o = items[idx[at - 1]];
+            if ((o.rows > o.cols ? o.rows : o.cols) >= len) break;
+            idx[at] = idx[at - 1];
+        }
+        idx[at] = i;
     }
-    return most ? most : 256;
+    return 0;
+}
+template <typename Item>
+size_t ns_workspace(const Item* items, int n) {
+    size_t most = 256;
+    for (int i = 0; i < n; ++i)
+        if (ns_check_shape("newton_schulz", i, items[i].count, items[i].rows, items[i].cols)) return 0;
+    ns_rounds(items, n, [&](const NsPlan& pl, const int*, int) {
+        if (pl.bytes > most) most = pl.bytes;
+        return 0;
+    });
+    return most;
 }
 
 }  // namespace
@@ -622,28 +827,17 @@ int s3d_launch_orthogonalize(const S3dOrthoItem* items, int n, const S3dNsArgs* 
     }
     const size_t need = ns_workspace(items, n);
     S3D_REQUIRE(workspace && bytes >= need && ((uintptr_t)workspace & 15) == 0, "%s: the workspace needs %zu bytes, 16-byte aligned", who, need);
-    int count[NS_ITEMS], rows[NS_ITEMS], cols[NS_ITEMS], k = 0;
-    NsPlan pl;
-    NsPtrs p;
-    memset(&p, 0, sizeof(p));
-    for (int i = 0; i <= n; ++i) {
-        if (k == NS_ITEMS || (i == n && k > 0)) {
-            ns_plan(pl, k, count, rows, cols);
-            int rc;
-            if (a->x_bf16) rc = a->out_bf16 ? ns_run<SRC_BF16, EPI_OUT_BF16>(pl, p, *a, nullptr, workspace, s) : ns_run<SRC_BF16, EPI_OUT_F32>(pl, p, *a, nullptr, workspace, s);
-            else rc = a->out_bf16 ? ns_run<SRC_F32, EPI_OUT_BF16>(pl, p, *a, nullptr, workspace, s) : ns_run<SRC_F32, EPI_OUT_F32>(pl, p, *a, nullptr, workspace, s);
-            if (rc) return rc;
-            k = 0;
+    return ns_rounds(items, n, [&](NsPlan& pl, const int* idx, int k) {
+        NsPtrs p;
+        memset(&p, 0, sizeof(p));
+        for (int j = 0; j < k; ++j) {
+            const S3dOrthoItem& q = items[idx[j]];
+            p.x[j] = q.x; p.xs[j] = q.x_stride; p.xld[j] = q.x_ld;
+            p.o[j] = q.out; p.os[j] = q.out_stride; p.old[j] = q.out_ld;
         }
-        if (i == n) break;
-        const S3dOrthoItem& q = items[i];
-        if (q.count == 0 || q.rows == 0 || q.cols == 0) continue;
-        count[k] = q.count; rows[k] = q.rows; cols[k] = q.cols;
-        p.x[k] = q.x; p.xs[k] = q.x_stride; p.xld[k] = q.x_ld;
-        p.o[k] = q.out; p.os[k] = q.out_stride; p.old[k] = q.out_ld;
-        ++k;
-    }
-    return 0;
+        if (a->x_bf16) return a->out_bf16 ? ns_run<SRC_BF16, EPI_OUT_BF16>(pl, p, *a, nullptr, workspace, s) : ns_run<SRC_BF16, EPI_OUT_F32>(pl, p, *a, nullptr, workspace, s);
+        return a->out_bf16 ? ns_run<SRC_F32, EPI_OUT_BF16>(pl, p, *a, nullptr, workspace, s) : ns_run<SRC_F32, EPI_OUT_F32>(pl, p, *a, nullptr, workspace, s);
+    });
 }
 
 int s3d_launch_muon(const S3dMuonItem* items, int n, const S3dNsArgs* a, const float* hyper, void* workspace, size_t bytes, hipStream_t s) {
@@ -665,25 +859,16 @@ int s3d_launch_muon(const S3dMuonItem* items, int n, const S3dNsArgs* a, const f
     }
     const size_t need = ns_workspace(items, n);
     S3D_REQUIRE(workspace && bytes >= need && ((uintptr_t)workspace & 15) == 0, "%s: the workspace needs %zu bytes, 16-byte aligned", who, need);
-    int count[NS_ITEMS], rows[NS_ITEMS], cols[NS_ITEMS], k = 0;
-    NsPlan pl;
-    NsPtrs p;
-    memset(&p, 0, sizeof(p));
-    for (int i = 0; i <= n; ++i) {
-        if (k == NS_ITEMS || (i == n && k > 0)) {
-            ns_plan(pl, k, count, rows, cols);
-            if (int rc = ns_run<SRC_MUON, EPI_UPDATE>(pl, p, *a, hyper, workspace, s)) return rc;
-            k = 0;
+    return ns_rounds(items, n, [&](NsPlan& pl, const int* idx, int k) {
+        NsPtrs p;
+        memset(&p, 0, sizeof(p));
+        for (int j = 0; j < k; ++j) {
+            const S3dMuonItem& q = items[idx[j]];
+            p.x[j] = q.g; p.xs[j] = q.g_stride; p.xld[j] = q.g_ld;
+            p.o[j] = q.p; p.os[j] = q.p_stride; p.old[j] = q.p_ld;
+            p.m[j] = q.m; p.ms[j] = q.m_stride; p.mld[j] = q.m_ld;
+            p.hi[j] = q.hi; p.lo[j] = q.lo; p.scale[j] = q.scale;
         }
-        if (i == n) break;
-        const S3dMuonItem& q = items[i];
-        if (q.count == 0 || q.rows == 0 || q.cols == 0) continue;
-        count[k] = q.count; rows[k] = q.rows; cols[k] = q.cols;
-        p.x[k] = q.g; p.xs[k] = q.g_stride; p.xld[k] = q.g_ld;
-        p.o[k] = q.p; p.os[k] = q.p_stride; p.old[k] = q.p_ld;
-        p.m[k] = q.m; p.ms[k] = q.m_stride; p.mld[k] = q.m_ld;
-        p.hi[k] = q.hi; p.lo[k] = q.lo; p.scale[k] = q.scale;
-        ++k;
-    }
-    return 0;
+        return ns_run<SRC_MUON, EPI_UPDATE>(pl, p, *a, hyper, workspace, s);
+    });
 }

@@ -124,17 +124,25 @@ def cross_entropy(logits, target, weight=None, grad_scale=1.0):
 # ---------------------------------------------------------------------------------------------- head norm + position rotation
 def _same_device(who, *tensors):
     """All tensors on the CURRENT device: the call is enqueued on the current stream of it."""
-    dev = torch.device('cuda', torch.cuda.current_device()) if torch.cuda.is_available() else None
+    cur = None
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f'{who}: every tensor must be on the current device ({dev}), got one on {t.device}')
+        if t is None:
+            continue
+        if t.is_cuda and cur is None:
+            cur = torch.cuda.current_device()
+        if not t.is_cuda or t.get_device() != cur:
+            raise ValueError(f'{who}: every tensor must be on the current device, got one on {t.device}')
 
 
 def _plane(who, name, t, rows, width):
-    """A [rows, >= width] bf16 plane with unit column stride; returns its row pitch."""
-    if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
+    """A [rows, width] bf16 plane with contiguous rows; returns its row pitch."""
+    if t.dtype != torch.bfloat16 or t.shape != (rows, width) or t.stride(1) != 1:
         raise ValueError(f'{who}: {name} must be a bfloat16 [{rows}, {width}] tensor with contiguous rows, got {t.dtype} {tuple(t.shape)} {t.stride()}')
     return t.stride(0) if rows > 1 else max(t.stride(0), width)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 def rope_table(coords, hd, base=10000.0):
@@ -156,35 +164,37 @@ def rope_table(coords, hd, base=10000.0):
     return ang.cos().float(), ang.sin().float()
 
 
-def _qk_args(who, qkv_hi, qkv_lo, H, hd, Hkv, q_gain, k_gain, rope, pos, st, eps, interleaved, others):
+def _qk_args(who, qkv_hi, qkv_lo, H, hd, Hkv, q_gain, k_gain, rope, pos, st, eps, interleaved):
+    """The checked argument block of either direction, rows, width and the planes' row pitch."""
     Hkv = H if Hkv is None else Hkv
     if qkv_hi.dim() != 2:
         raise ValueError(f'{who}: qkv must be [rows, (H + 2 Hkv) hd], got {tuple(qkv_hi.shape)}')
     rows, W = qkv_hi.shape[0], (H + 2 * Hkv) * hd
-    cos, sin = rope if rope is not None else (None, None)
-    _same_device(who, qkv_hi, qkv_lo, q_gain, k_gain, cos, sin, pos, *others)
     ld = _plane(who, 'qkv_hi', qkv_hi, rows, W)
     if qkv_lo is not None and _plane(who, 'qkv_lo', qkv_lo, rows, W) != ld:
         raise ValueError(f'{who}: the planes of a pair need the same row pitch')
-    for name, g in (('q_gain', q_gain), ('k_gain', k_gain)):
-        if g is not None and (g.dtype != torch.float32 or tuple(g.shape) != (hd,) or not g.is_contiguous()):
-            raise ValueError(f'{who}: {name} must be a contiguous float32 [{hd}] tensor')
+    for g in (q_gain, k_gain):
+        if g is not None and (g.dtype != torch.float32 or g.shape != (hd,) or not g.is_contiguous()):
+            raise ValueError(f'{who}: q_gain and k_gain must be contiguous float32 [{hd}] tensors')
+    cos, sin = rope if rope is not None else (None, None)
     T = 0
     if cos is not None:
         T = cos.shape[0]
         for t in (cos, sin):
-            if t.dtype != torch.float32 or tuple(t.shape) != (T, hd // 2) or not t.is_contiguous():
+            if t.dtype != torch.float32 or t.shape != (T, hd // 2) or not t.is_contiguous():
                 raise ValueError(f'{who}: the rotation tables must be contiguous float32 [T, {hd // 2}] tensors')
-    if pos is not None and (pos.dtype != torch.int32 or tuple(pos.shape) != (rows,) or not pos.is_contiguous()):
+    if pos is not None and (pos.dtype != torch.int32 or pos.shape != (rows,) or not pos.is_contiguous()):
         raise ValueError(f'{who}: pos must be a contiguous int32 [{rows}] tensor')
-    a = L.fill(L.S3dQkNormArgs(), qkv_hi=qkv_hi, qkv_lo=qkv_lo, ld=ld, rows=rows, H=H, Hkv=Hkv, hd=hd, eps=eps, q_gain=q_gain, k_gain=k_gain,
-               cos_t=cos, sin_t=sin, T=T, st=st, pos=pos, interleaved=1 if interleaved else 0)
+    a = L.S3dQkNormArgs(qkv_hi=qkv_hi.data_ptr(), qkv_lo=_addr(qkv_lo), ld=ld, rows=rows, H=H, Hkv=Hkv, hd=hd, eps=eps, q_gain=_addr(q_gain),
+                        k_gain=_addr(k_gain), cos_t=_addr(cos), sin_t=_addr(sin), T=T, st=st, pos=_addr(pos), interleaved=1 if interleaved else 0)
     return a, rows, W
 
 
 def _pair_out(who, name, out, like_hi, like_lo, rows, W):
-    hi, lo = out if out is not None else (torch.empty_like(like_hi, memory_format=torch.contiguous_format),
-                                          None if like_lo is None else torch.empty_like(like_lo, memory_format=torch.contiguous_format))
+    if out is None:
+        return (torch.empty_like(like_hi, memory_format=torch.contiguous_format),
+                None if like_lo is None else torch.empty_like(like_lo, memory_format=torch.contiguous_format), W)
+    hi, lo = out
     ld = _plane(who, name, hi, rows, W)
     if lo is not None and _plane(who, name + ' (low plane)', lo, rows, W) != ld:
         raise ValueError(f'{who}: the planes of a pair need the same row pitch')
@@ -197,10 +207,11 @@ def qk_norm_rope_fwd(qkv_hi, qkv_lo, H, hd, *, Hkv=None, q_gain=None, k_gain=Non
     pos [rows] int32 table rows (outside the table: not rotated) or None: row r takes (r // st) % T.  out = (hi, lo) to write into, which may
     be the input planes; -> (out_hi, out_lo)."""
     who = 'qk_norm_rope_fwd'
-    a, rows, W = _qk_args(who, qkv_hi, qkv_lo, H, hd, Hkv, q_gain, k_gain, rope, pos, st, eps, interleaved, out or ())
-    hi, lo, ld = _pair_out(who, 'out', out, qkv_hi, qkv_lo, rows, W)
-    L.fill(a, out_hi=hi, out_lo=lo, ldo=ld)
+    _same_device(who, qkv_hi, qkv_lo, q_gain, k_gain, pos, *(rope or ()), *(out or ()))
+    a, rows, W = _qk_args(who, qkv_hi, qkv_lo, H, hd, Hkv, q_gain, k_gain, rope, pos, st, eps, interleaved)
+    hi, lo, a.ldo = _pair_out(who, 'out', out, qkv_hi, qkv_lo, rows, W)
     if rows:
+        a.out_hi, a.out_lo = hi.data_ptr(), _addr(lo)
         L.check(L.lib().s3d_qk_norm_rope_fwd(ctypes.byref(a), L.current_stream()), who)
     return hi, lo
 
@@ -210,23 +221,25 @@ def qk_norm_rope_bwd(dout_hi, dout_lo, qkv_hi, qkv_lo, H, hd, *, Hkv=None, q_gai
     """Backward of qk_norm_rope_fwd: dout planes (gradient of its output) and the INPUT qkv planes of the forward -> (dqkv_hi, dqkv_lo, dq_gain,
     dk_gain).  out = (hi, lo) to write dqkv into (may be the dout planes); gain_grads = (dq, dk) to ADD the gains' gradients to."""
     who = 'qk_norm_rope_bwd'
-    dq, dk = gain_grads if gain_grads is not None else (None, None)
-    a, rows, W = _qk_args(who, qkv_hi, qkv_lo, H, hd, Hkv, q_gain, k_gain, rope, pos, st, eps, interleaved, (dout_hi, dout_lo, dq, dk) + tuple(out or ()))
-    lddo = _plane(who, 'dout_hi', dout_hi, rows, W)
-    if dout_lo is not None and _plane(who, 'dout_lo', dout_lo, rows, W) != lddo:
+    _same_device(who, qkv_hi, qkv_lo, dout_hi, dout_lo, q_gain, k_gain, pos, *(rope or ()), *(out or ()), *(gain_grads or ()))
+    a, rows, W = _qk_args(who, qkv_hi, qkv_lo, H, hd, Hkv, q_gain, k_gain, rope, pos, st, eps, interleaved)
+    a.lddo = _plane(who, 'dout_hi', dout_hi, rows, W)
+    if dout_lo is not None and _plane(who, 'dout_lo', dout_lo, rows, W) != a.lddo:
         raise ValueError(f'{who}: the planes of a pair need the same row pitch')
-    hi, lo, ld = _pair_out(who, 'out', out, dout_hi, dout_lo, rows, W)
+    hi, lo, a.lddq = _pair_out(who, 'out', out, dout_hi, dout_lo, rows, W)
     if gain_grads is None:
-        dq, dk = torch.empty(2, hd, dtype=torch.float32, device=qkv_hi.device)
-    for g in (dq, dk):
-        if g.dtype != torch.float32 or tuple(g.shape) != (hd,) or not g.is_contiguous():
-            raise ValueError(f'{who}: the gains\' gradients must be contiguous float32 [{hd}] tensors')
-    lib = L.lib()
-    blocks = lib.s3d_qk_norm_blocks(rows, a.H, a.Hkv, hd)
-    part = torch.empty(max(blocks, 1) * 2 * hd, dtype=torch.float32, device=qkv_hi.device)
-    L.fill(a, dout=dout_hi, dout_lo=dout_lo, lddo=lddo, dqkv=hi, dqkv_lo=lo, lddq=ld, dq_gain=dq, dk_gain=dk, accumulate=0 if gain_grads is None else 1,
-           partial=part, partial_blocks=blocks)
+        dq, dk = (torch.empty(hd, dtype=torch.float32, device=qkv_hi.device) for _ in range(2))
+    else:
+        dq, dk = gain_grads
+        for g in (dq, dk):
+            if g.dtype != torch.float32 or g.shape != (hd,) or not g.is_contiguous():
+                raise ValueError(f'{who}: the gains\' gradients must be contiguous float32 [{hd}] tensors')
     if rows:
+        lib = L.lib()
+        a.partial_blocks = lib.s3d_qk_norm_blocks(rows, a.H, a.Hkv, hd)
+        part = torch.empty(a.partial_blocks * 2 * hd, dtype=torch.float32, device=qkv_hi.device)
+        a.dout, a.dout_lo, a.dqkv, a.dqkv_lo = dout_hi.data_ptr(), _addr(dout_lo), hi.data_ptr(), _addr(lo)
+        a.dq_gain, a.dk_gain, a.accumulate, a.partial = dq.data_ptr(), dk.data_ptr(), int(gain_grads is not None), part.data_ptr()
         L.check(lib.s3d_qk_norm_rope_bwd(ctypes.byref(a), L.current_stream()), who)
     elif gain_grads is None:
         dq.zero_()
@@ -252,7 +265,7 @@ def _matrices(who, name, t, dtypes):
 
 def _ns_args(steps, coefficients, eps, **kw):
     a, b, c = coefficients
-    return L.fill(L.S3dNsArgs(), steps=steps, a=a, b=b, c=c, eps=eps, **kw)
+    return L.S3dNsArgs(steps=steps, a=a, b=b, c=c, eps=eps, **kw)
 
 
 def orthogonalize(x, *, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dtype=None, out=None):
@@ -268,12 +281,12 @@ def orthogonalize(x, *, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dty
     elif out.shape != x.shape or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f'{who}: out must have the shape of x and the requested type')
     _, _, _, os_, old = _matrices(who, 'out', out, types)
-    it = (L.S3dOrthoItem * 1)(L.fill(L.S3dOrthoItem(), x=x, x_stride=xs, x_ld=xld, out=out, out_stride=os_, out_ld=old, count=n, rows=r, cols=c))
+    it = L.S3dOrthoItem(x=x.data_ptr(), x_stride=xs, x_ld=xld, out=out.data_ptr(), out_stride=os_, out_ld=old, count=n, rows=r, cols=c)
     a = _ns_args(steps, coefficients, eps, x_bf16=int(x.dtype == torch.bfloat16), out_bf16=int(out.dtype == torch.bfloat16))
     lib = L.lib()
-    size = lib.s3d_orthogonalize_workspace_bytes(it, 1, ctypes.byref(a))
+    size = lib.s3d_orthogonalize_workspace_bytes(ctypes.byref(it), 1, ctypes.byref(a))
     ws = torch.empty(max(size, 16), dtype=torch.uint8, device=x.device)
-    L.check(lib.s3d_orthogonalize(it, 1, ctypes.byref(a), L.ptr(ws), size, L.current_stream()), who)
+    L.check(lib.s3d_orthogonalize(ctypes.byref(it), 1, ctypes.byref(a), ws.data_ptr(), size, L.current_stream()), who)
     return out
 
 
@@ -312,10 +325,10 @@ def muon_step(params, grads, momenta, hyper, *, planes=None, nesterov=True, step
             for t in (hi, lo):
                 if t.shape != p.shape or _matrices(who, f'planes[{i}]', t, (torch.bfloat16,))[3:] != (ps, pld):
                     raise ValueError(f'{who}: the planes of parameter {i} must be laid out like it')
-        L.fill(items[i], p=p, p_stride=ps, p_ld=pld, g=g, g_stride=gs, g_ld=gld, m=m, m_stride=ms, m_ld=mld, hi=hi, lo=lo, count=n, rows=r, cols=c,
-               scale=muon_scale(scale, r, c) if r and c else 0.0)
+        items[i] = L.S3dMuonItem(p=p.data_ptr(), p_stride=ps, p_ld=pld, g=g.data_ptr(), g_stride=gs, g_ld=gld, m=m.data_ptr(), m_stride=ms, m_ld=mld,
+                                 hi=_addr(hi), lo=_addr(lo), count=n, rows=r, cols=c, scale=muon_scale(scale, r, c) if r and c else 0.0)
     a = _ns_args(steps, coefficients, eps, nesterov=int(bool(nesterov)), zero_grad=int(bool(zero_grad)))
     lib = L.lib()
     size = lib.s3d_muon_workspace_bytes(items, len(params), ctypes.byref(a))
     workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=hyper.device)
-    L.check(lib.s3d_muon_step(items, len(params), ctypes.byref(a), L.ptr(hyper), L.ptr(workspace), size, L.current_stream()), who)
+    L.check(lib.s3d_muon_step(items, len(params), ctypes.byref(a), hyper.data_ptr(), workspace.data_ptr(), size, L.current_stream()), who)
