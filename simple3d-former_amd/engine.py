@@ -17,6 +17,7 @@ import numpy as np
 import torch
 
 from . import _lib as L
+from . import ops
 
 BACKBONES = {  # models/vit_3d_2d_pretrain.py:279-325 -- deit_base is built with num_heads=3 (reference quirk)
     'deit_tiny_patch16_224': dict(embed_dim=192, depth=12, num_heads=3),
@@ -384,6 +385,7 @@ class VoxelEngine:
         # group_embed encoder-layer dropout: 0 = eval mode; set_dropout(0.1) = the reference's training mode (hash-based masks)
         self.dropout_p = 0.0
         self.dropout_seed = torch.zeros(1, dtype=torch.int64, device=self.device)
+        self.muon = None                           # set_muon: matrix parameters by s3d_muon_step, the others by Adam
 
     # ------------------------------------------------------------------ parameters
     def _build_param_tables(self):
@@ -468,6 +470,28 @@ class VoxelEngine:
         st[:7] = np.array([lr, betas[0], betas[1], eps, grad_scale, 0.0, 0.0], dtype=np.float32).view(np.int32)
         st[7] = cur_step
         self.adam_state.copy_(torch.from_numpy(st))
+
+    def set_muon(self, lr=None, momentum=None, weight_decay=None, grad_scale=None, *, nesterov=True, steps=5, coefficients=ops.NS_COEFFICIENTS,
+                 scale='match_rms_adamw'):
+        """From now on train_step / optimizer_step update the matrix parameters of the transformer (attn.qkv, attn.proj, mlp.fc1, mlp.fc2 weights of
+        every block, the four of group_embed) with orthogonalised momentum (s3d_muon_step; the Adam arena m holds the momentum) and everything
+        else with Adam as before (set_optimizer).  lr, momentum, weight_decay and grad_scale live on the device, so a captured step follows
+        them; left at None they keep their value (at first 1e-3, 0.95, 0, 1).  The rest is baked into captured graphs.  unset_muon() goes back.
+        Single process: the data-parallel trainers update slices of the arena with Adam and refuse."""
+        if not hasattr(self, '_muon_hyper'):
+            self._muon_hyper = torch.tensor([1e-3, 0.95, 0.0, 1.0], dtype=torch.float32, device=self.device)
+        for i, v in enumerate((lr, momentum, weight_decay, grad_scale)):
+            if v is not None:
+                self._muon_hyper[i:i + 1].fill_(float(v))
+        muon = (bool(nesterov), int(steps), tuple(float(c) for c in coefficients), scale)
+        if muon != self.muon:
+            self.capture_epoch += 1                # trainers holding their own captures re-capture (and refuse); this engine's cache is keyed by it
+        self.muon = muon
+
+    def unset_muon(self):
+        if self.muon is not None:
+            self.capture_epoch += 1
+        self.muon = None
 
     def set_dropout(self, p, seed=None):
         """Dropout of nn.TransformerEncoderLayer inside group_embed (vit_3d_2d_pretrain.py:381; p = 0.1 when model.train()).
@@ -928,9 +952,59 @@ class VoxelEngine:
         L.check(lib.s3d_token_grads(ctypes.byref(pg), s), 'token grads')
 
     # ------------------------------------------------------------------ optimizer
+    def muon_stacks(self):
+        """The matrix parameters as stacks of equal matrices, one per block: [(key of the first, count, rows, cols, stride in floats)]."""
+        a, out = self.arena, []
+        for k in ('attn.qkv.weight', 'attn.proj.weight', 'mlp.fc1.weight', 'mlp.fc2.weight'):
+            first = f'blocks.0.{k}'
+            stride = a.offsets[f'blocks.1.{k}'] - a.offsets[first] if self.depth > 1 else 0
+            assert all(a.offsets[f'blocks.{i}.{k}'] == a.offsets[first] + i * stride for i in range(self.depth)), 'blocks are laid out alike'
+            out.append((first, self.depth, *a.shapes[first], stride))
+        if self.group:
+            for k in ('self_attn.in_proj_weight', 'self_attn.out_proj.weight', 'linear1.weight', 'linear2.weight'):
+                out.append(('group_embed.' + k, 1, *a.shapes['group_embed.' + k], 0))
+        return out
+
+    def _adam_ranges(self, skip, zero_grad):
+        """Adam on everything outside the [offset, count) ranges of `skip` (after s3d_adam_begin), up to 64 gaps a launch."""
+        a, rest, pos = self.arena, [], 0
+        for off, cnt in sorted(skip):
+            if off > pos:
+                rest.append((pos, off - pos))
+            pos = _round_up(off + cnt, 8)          # the pad behind a parameter is zero and stays zero
+        if pos < a.numel:
+            rest.append((pos, a.numel - pos))
+        for i in range(0, len(rest), 64):
+            part = rest[i:i + 64]
+            flat = (ctypes.c_long * (2 * len(part)))(*[v for r in part for v in r])
+            L.check(self.lib.s3d_adam_apply_ranges(L.ptr(a.p), L.ptr(a.g), L.ptr(a.m), L.ptr(a.v), L.ptr(a.hi), L.ptr(a.lo), flat, len(part),
+                                                   L.ptr(self.adam_state), 1 if zero_grad else 0, L.current_stream()), 'adam ranges')
+
+    def muon_step(self, zero_grad=True):
+        """optimizer.step() with orthogonalised momentum for the matrix parameters and Adam for the others (after set_muon)."""
+        if self.muon is None:
+            raise RuntimeError('muon_step: call set_muon first')
+        nesterov, steps, coefficients, scale = self.muon
+        a, stacks = self.arena, self.muon_stacks()
+        self.adam_begin()
+        stack = lambda t: [t.as_strided((n, r, c), (stride, c, 1), a.offsets[k]) for k, n, r, c, stride in stacks]
+        ops.muon_step(stack(a.p), stack(a.g), stack(a.m), self._muon_hyper, planes=list(zip(stack(a.hi), stack(a.lo))), nesterov=nesterov, steps=steps,
+                      coefficients=coefficients, scale=scale, zero_grad=zero_grad)
+        self._adam_ranges([(a.offsets[k] + i * stride, r * c) for k, n, r, c, stride in stacks for i in range(n)], zero_grad)
+        self._refresh_conv_planes()
+
+    def optimizer_step(self, zero_grad=True):
+        """What train_step does behind the backward: muon_step after set_muon, adam_step otherwise."""
+        return self.adam_step(zero_grad) if self.muon is None else self.muon_step(zero_grad)
+
+    def _require_adam(self, who):
+        if self.muon is not None:
+            raise RuntimeError(f'{who}: set_muon is in effect (use optimizer_step, or unset_muon first): Adam would update the matrix parameters too')
+
     def adam_step(self, zero_grad=True, wire=None):
         """wire: bf16 tensor of the arena's layout holding the (all-reduced) gradient -- the data-parallel wire format; the
         fp32 gradient arena is then only zeroed."""
+        self._require_adam('adam_step')
         a = self.arena
         if wire is None:
             L.check(self.lib.s3d_adam_step(L.ptr(a.p), L.ptr(a.g), L.ptr(a.m), L.ptr(a.v), L.ptr(a.hi), L.ptr(a.lo),
@@ -950,6 +1024,7 @@ class VoxelEngine:
     def adam_apply(self, start, end, zero_grad=True, max_workgroups=0, wire=None):
         """Adam on the arena slice [start, end) on the current stream (gradients of the slice must be final there).  wire: the flat bf16
         gradient buffer of the data-parallel wire format (the slice's gradient is read from it, the fp32 arena only zeroed)."""
+        self._require_adam('adam_apply')
         a = self.arena
         off = lambda t, b: ctypes.c_void_p(t.data_ptr() + b * start)
         L.check(self.lib.s3d_adam_apply(off(a.p, 4), off(a.g, 4), None if wire is None else off(wire, 2), off(a.m, 4), off(a.v, 4),
@@ -971,14 +1046,14 @@ class VoxelEngine:
 
     # ------------------------------------------------------------------ fused training step
     def train_step(self, x, target, weight=None):
-        """zero_grad -> model(voxel) -> F.cross_entropy -> backward -> Adam  (train_cls_voxel.py:277-288), all on the
-        HIP path.  Gradients are zeroed by the previous step's Adam kernel.  Returns the loss as a device scalar."""
+        """zero_grad -> model(voxel) -> F.cross_entropy -> backward -> Adam  (train_cls_voxel.py:277-288; after set_muon: muon_step), all on the
+        HIP path.  Gradients are zeroed by the previous step's optimizer kernels.  Returns the loss as a device scalar."""
         B = x.shape[0]
         self.advance_dropout_seed()                       # fresh masks every step (device-side, graph-replay safe)
         loss = self.forward_loss(x, target, weight)
         n_slices = getattr(self, 'update_slices', UPDATE_OVERLAP)
-        if n_slices <= 0 or self.precise:
-            if getattr(self, 'adam_fill', ADAM_FILL) and not self.precise and not self.group and self.images is None and self.world_size == 1:
+        if n_slices <= 0 or self.precise or self.muon is not None:
+            if getattr(self, 'adam_fill', ADAM_FILL) and self.muon is None and not self.precise and not self.group and self.images is None and self.world_size == 1:
                 # optimizer.step() inside loss.backward(): the bookkeeping first, the GEMM parameters of block i + 1 on block i's launches,
                 # the rest in one launch at the end (bitwise the results of adam_step)
                 self.adam_begin()
@@ -999,7 +1074,7 @@ class VoxelEngine:
                 self.backward(B)
             finally:
                 self.grads_owned = False
-            self.adam_step(zero_grad=True)
+            self.optimizer_step(zero_grad=True)
             return loss
         main = torch.cuda.current_stream()
         if getattr(self, '_update_stream', None) is None:
@@ -1037,7 +1112,7 @@ class VoxelEngine:
         li = self.images.cross_entropy(Bi, img_target, grad_scale=lambda_weight)
         self.backward(B)
         self.images.backward(Bi)
-        self.adam_step(zero_grad=True)
+        self.optimizer_step(zero_grad=True)
         return lv + lambda_weight * li, lv, li
 
     def capture_train_step(self, B, weight=None):
@@ -1045,7 +1120,7 @@ class VoxelEngine:
         ws = self.workspace(B)                      # (may grow the shared attention-mask buffer: that clears the cache, see _ensure_attn_mask)
         mask = getattr(self, '_attn_mask', None) if self.group else None
         key = (B, None if weight is None else weight.data_ptr(), self.dropout_p, getattr(self, 'update_slices', UPDATE_OVERLAP), getattr(self, 'adam_fill', ADAM_FILL),
-               None if mask is None else mask.data_ptr(), self.backward_precision)     # model.train() / .eval() toggles keep both captures
+               None if mask is None else mask.data_ptr(), self.backward_precision, self.muon)     # model.train() / .eval() toggles keep both captures
         if key in self._graphs:
             return self._graphs[key]
         sx = torch.zeros(B, 1, self.V, self.V, self.V, dtype=torch.float32, device=self.device)
