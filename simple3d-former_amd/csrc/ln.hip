@@ -98,16 +98,16 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LnBwdArgs p, const Ad
                     const float4 w = *reinterpret_cast<const float4*>(p.gamma + col);
                     const float4 x = X[i][c], dy = DY[i][c];
                     xh[c] = make_float4((x.x - mean[i]) * rstd[i], (x.y - mean[i]) * rstd[i], (x.z - mean[i]) * rstd[i], (x.w - mean[i]) * rstd[i]);
-                    g[c] = make_float4(dy.x * w.x, dy.y * w.y, dy.z * w.z, dy.w * w.w);
-                    s1 += g[c].x + g[c].y + g[c].z + g[c].w;
-                    s2 += g[c].x * xh[c].x + g[c].y * xh[c].y + g[c].z * xh[c].z + g[c].w * xh[c].w;
+                    g[c] = ln_mul4(dy, w);
+                    s1 += fmaf(w.y, dy.y, g[c].x) + g[c].z + g[c].w;
+                    s2 += ln_dot4(xh[c], g[c]);
                     if (live) {
                         dg[c].x += dy.x * xh[c].x; dg[c].y += dy.y * xh[c].y; dg[c].z += dy.z * xh[c].z; dg[c].w += dy.w * xh[c].w;
                         db[c].x += dy.x; db[c].y += dy.y; db[c].z += dy.z; db[c].w += dy.w;
                     }
                 }
             }
-            s1 = wave_sum(s1) * inv_d;                  // (a division here is ~10 instructions on every lane, twice per row)
+            s1 = ln_mul(wave_sum(s1), inv_d);           // (a division here is ~10 instructions on every lane, twice per row)
             s2 = wave_sum(s2) * inv_d;
             if (!live) continue;                          // wave-uniform
 #pragma unroll

@@ -4,6 +4,25 @@
 #pragma once
 #include "common.h"
 
+// The sums below say which products are rounded and which are fused.  Left to itself the compiler chooses, and chooses differently
+// with its flags; long training runs in an unstable regime (one that multiplies 1e-7 to 1e-3) follow the last bit.
+__device__ __forceinline__ float ln_sq4(const float a, const float b, const float c, const float d) {
+#pragma clang fp contract(off)
+    return a * a + b * b + c * c + d * d;
+}
+__device__ __forceinline__ float ln_dot4(const float4 a, const float4 b) {
+#pragma clang fp contract(off)
+    return fmaf(a.x, b.x, a.y * b.y) + a.z * b.z + a.w * b.w;
+}
+__device__ __forceinline__ float ln_mul(const float a, const float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+__device__ __forceinline__ float4 ln_mul4(const float4 a, const float4 b) {
+#pragma clang fp contract(off)
+    return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w);
+}
+
 template <int MC>
 __device__ __forceinline__ void ln_row_finish(const float4 (&v)[MC], const int lane, const int D, const float eps,
                                               const float* __restrict__ gamma, const float* __restrict__ beta, float* mean_out,
@@ -19,7 +38,7 @@ __device__ __forceinline__ void ln_row_finish(const float4 (&v)[MC], const int l
         const int col = c * 256 + lane * 4;
         if (col < D) {
             const float a = v[c].x - mean, b = v[c].y - mean, cc = v[c].z - mean, d = v[c].w - mean;
-            q += a * a + b * b + cc * cc + d * d;
+            q += ln_sq4(a, b, cc, d);
         }
     }
     const float rstd = rsqrtf(wave_sum(q) * inv_d + eps);
