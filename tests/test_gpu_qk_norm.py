@@ -173,6 +173,30 @@ def test_strided_rows_in_place_and_memory_around():
     assert bool((buf == 7.0).all())
 
 
+def test_pairs_and_plain_planes_mixed():
+    """A pair into one plane and one plane into a pair, forward and backward: the same values as with the planes alike."""
+    rows, H, hd = 21, 2, 64
+    hi, lo = make(rows, H, H, hd, True)
+    d, dlo = make(rows, H, H, hd, True, seed=1)
+    rope = table(rows, hd)
+    new = lambda: torch.empty_like(hi)
+    pair = ops.qk_norm_rope_fwd(hi, lo, H, hd, rope=rope)
+    one, none = ops.qk_norm_rope_fwd(hi, lo, H, hd, rope=rope, out=(new(), None))
+    V = 2 * H * hd                                                       # queries and keys: the hi plane is the value rounded to bf16.  Values: the
+    assert none is None and torch.equal(one[:, :V], pair[0][:, :V])      # planes bit for bit, or their sum rounded (not hi where lo is half a step)
+    assert torch.equal(one[:, V:], (hi.float() + lo.float()).to(torch.bfloat16)[:, V:])
+    a, b = ops.qk_norm_rope_fwd(hi, None, H, hd, rope=rope, out=(new(), new()))
+    ref, mag = oracle(hi.double(), H, H, hd, None, None, angles(rope, torch.arange(rows, device=DEV)), False)
+    assert bool(((whole(a, b) - ref).abs() <= ref.abs() * 2.0 ** -16 + 32 * 2.0 ** -24 * mag).all())
+    assert bool((b[:, V:] == 0).all()) and torch.equal(a[:, V:], hi[:, V:])
+    full = ops.qk_norm_rope_bwd(d, dlo, hi, lo, H, hd, rope=rope)
+    one = ops.qk_norm_rope_bwd(d, dlo, hi, lo, H, hd, rope=rope, out=(new(), None))
+    assert torch.equal(one[0][:, :V], full[0][:, :V]) and torch.equal(one[2], full[2]) and torch.equal(one[3], full[3])
+    full = ops.qk_norm_rope_bwd(d, None, hi, lo, H, hd, rope=rope, out=(new(), new()))
+    one = ops.qk_norm_rope_bwd(d, None, hi, lo, H, hd, rope=rope)
+    assert one[1] is None and torch.equal(one[0], full[0]) and bool((full[1][:, V:] == 0).all())
+
+
 def test_zero_rows_no_rows_and_special_values():
     H, hd = 2, 48
     W = 3 * H * hd
