@@ -256,9 +256,10 @@ int s3d_attention_bwd(const S3dAttnArgs* args, s3d_stream_t stream);
  *   pos             [rows] table row of every token, or NULL: row r takes table row (r / st) % T (st = 1: sequences of T tokens one after the
  *                   other; st = number of sequences: token-major rows).  A position outside [0, T) leaves the token unrotated (class tokens: -1).
  *   *_lo            optional low planes of split-bf16 tensors; the gains may be NULL (= 1).
- * out may be qkv itself (same pointers and pitch; the value heads are then not touched).  For a backward pass keep the input qkv.
+ * out may be qkv itself (same pointers and pitch; the value heads are then not touched); any other overlap of what is written is refused.  For a
+ * backward pass keep the input qkv.
  * Backward: dout = gradient of out; dqkv (may be dout itself) = gradient of qkv; dq_gain / dk_gain [hd] are stored, or added to when
- * `accumulate`; they are also computed when the gains are NULL.  partial = scratch of partial_blocks >= s3d_qk_norm_blocks(..) times 2 * hd
+ * `accumulate`; they are also computed when the gains are NULL, and may not be one tensor.  partial = scratch of partial_blocks >= s3d_qk_norm_blocks(..) times 2 * hd
  * floats.  No atomics: bitwise reproducible. */
 typedef struct S3dQkNormArgs {
     const uint16_t* qkv_hi; const uint16_t* qkv_lo; long ld;
@@ -421,7 +422,8 @@ int s3d_adam_step_wire(float* p, float* g, const uint16_t* g_wire, float* m, flo
  * worked transposed): every singular value s becomes a s + b s^3 + c s^5, the singular vectors stay.  A stack item is `count` matrices
  * [rows][cols] of one shape: matrix i of a tensor at + i * stride, row pitch ld (elements); any sizes, no alignment beyond the element's;
  * items with a zero size are skipped.  Products are taken on pairs of fp16 planes with fp32 accumulation (fp32-class, csrc/muon.hip).
- * Non-finite entries make that matrix's result NaN.  Calls are bitwise reproducible.
+ * Non-finite entries make that matrix's result NaN.  Calls are bitwise reproducible.  Tensors that are written may share no element with another item's
+ * (blocks of one matrix and matrices interleaved in one arena are told apart; other overlapping layouts are refused).
  * workspace: device scratch of at least the size the *_workspace_bytes call gives for the SAME items (16-byte aligned; contents are
  * neither expected nor kept; two calls that may overlap in time need two).  steps 1 .. 32; coefficients under which a singular value in
  * [0, 1] would grow past 64 are refused; eps >= 1e-30. */

@@ -15,12 +15,15 @@
 // instructions.  fp16 planes rather than bf16: all entries are bounded by the spectral norm, so the exponent range is not needed and
 // the six extra bits are.
 #include <math.h>
+#include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "kernels.h"
 #include "kmajor.h"
+#include "ranges.h"
 
 namespace {
 
@@ -809,6 +812,32 @@ size_t ns_workspace(const Item* items, int n) {
     return most;
 }
 
+// No tensor that is written may share elements with another one: the workgroups of a launch run in any order, and stacks beyond the sixteenth in
+// later launches.  Sorted by address, each compared with those that begin inside it.
+struct NsRanges {
+    MatRange* v;
+    long n = 0;
+    explicit NsRanges(long most) : v((MatRange*)malloc(sizeof(MatRange) * (most > 0 ? most : 1))) {}
+    ~NsRanges() { free(v); }
+    NsRanges(const NsRanges&) = delete;
+    NsRanges& operator=(const NsRanges&) = delete;
+    void add(const void* p, int size, long stride, long ld, int count, int rows, int cols, bool write, int item) {
+        v[n++] = MatRange{(uintptr_t)p, size, stride, ld, count, rows, cols, write, item};
+    }
+    // same_item: also tensors of one item
+    int check(const char* who, bool same_item) {
+        std::sort(v, v + n, [](const MatRange& a, const MatRange& b) { return a.at < b.at; });
+        for (long i = 0; i < n; ++i) {
+            const uintptr_t end = v[i].end();
+            for (long j = i + 1; j < n && v[j].at < end; ++j) {
+                if (!(v[i].write || v[j].write) || (!same_item && v[i].item == v[j].item)) continue;
+                S3D_REQUIRE(!ranges_meet(v[i], v[j]), "%s: a tensor of item %d that is written shares memory with one of item %d", who, v[i].item, v[j].item);
+            }
+        }
+        return 0;
+    }
+};
+
 }  // namespace
 
 size_t s3d_ortho_workspace(const S3dOrthoItem* items, int n) { return ns_workspace(items, n); }
@@ -828,6 +857,15 @@ int s3d_launch_orthogonalize(const S3dOrthoItem* items, int n, const S3dNsArgs* 
     }
     const size_t need = ns_workspace(items, n);
     S3D_REQUIRE(workspace && bytes >= need && ((uintptr_t)workspace & 15) == 0, "%s: the workspace needs %zu bytes, 16-byte aligned", who, need);
+    NsRanges used(2L * n);
+    S3D_REQUIRE(used.v, "%s: no host memory for %d items", who, n);
+    for (int i = 0; i < n; ++i) {
+        const S3dOrthoItem& q = items[i];
+        if (q.count == 0 || q.rows == 0 || q.cols == 0) continue;
+        if (q.x_stride >= 0) used.add(q.x, a->x_bf16 ? 2 : 4, q.x_stride, q.x_ld, q.count, q.rows, q.cols, false, i);
+        used.add(q.out, a->out_bf16 ? 2 : 4, q.out_stride, q.out_ld, q.count, q.rows, q.cols, true, i);
+    }
+    if (int rc = used.check(who, false)) return rc;
     return ns_rounds(items, n, [&](NsPlan& pl, const int* idx, int k) {
         NsPtrs p;
         memset(&p, 0, sizeof(p));
@@ -860,6 +898,20 @@ int s3d_launch_muon(const S3dMuonItem* items, int n, const S3dNsArgs* a, const f
     }
     const size_t need = ns_workspace(items, n);
     S3D_REQUIRE(workspace && bytes >= need && ((uintptr_t)workspace & 15) == 0, "%s: the workspace needs %zu bytes, 16-byte aligned", who, need);
+    NsRanges used(5L * n);
+    S3D_REQUIRE(used.v, "%s: no host memory for %d items", who, n);
+    for (int i = 0; i < n; ++i) {
+        const S3dMuonItem& q = items[i];
+        if (q.count == 0 || q.rows == 0 || q.cols == 0) continue;
+        used.add(q.p, 4, q.p_stride, q.p_ld, q.count, q.rows, q.cols, true, i);
+        used.add(q.m, 4, q.m_stride, q.m_ld, q.count, q.rows, q.cols, true, i);
+        used.add(q.g, 4, q.g_stride, q.g_ld, q.count, q.rows, q.cols, a->zero_grad != 0, i);
+        if (q.hi) {
+            used.add(q.hi, 2, q.p_stride, q.p_ld, q.count, q.rows, q.cols, true, i);
+            used.add(q.lo, 2, q.p_stride, q.p_ld, q.count, q.rows, q.cols, true, i);
+        }
+    }
+    if (int rc = used.check(who, true)) return rc;
     return ns_rounds(items, n, [&](NsPlan& pl, const int* idx, int k) {
         NsPtrs p;
         memset(&p, 0, sizeof(p));

@@ -11,6 +11,7 @@
 // key or the value heads of a range of rows (blockIdx.y): one gain and one gain gradient in registers, no divergence, and three times the
 // workgroups when there are few rows.
 #include "kernels.h"
+#include "ranges.h"
 
 namespace {
 
@@ -304,6 +305,18 @@ int check(const S3dQkNormArgs& a, bool bwd) {
         S3D_REQUIRE(a.dq_gain && a.dk_gain, "%s: dq_gain and dk_gain must be set", who);
         const int need = s3d_qk_norm_blocks(a.rows, a.H, a.Hkv, a.hd);
         S3D_REQUIRE(a.partial && a.partial_blocks >= need, "%s: partial needs %d blocks", who, need);
+        S3D_REQUIRE(a.dq_gain + a.hd <= a.dk_gain || a.dk_gain + a.hd <= a.dq_gain, "%s: dq_gain and dk_gain overlap (one gain for both: add the two)", who);
+    }
+    if (a.rows > 0) {
+        // what is written may be what is read in place (same plane and pitch: every element is read and written by one lane), never a shifted part of it
+        const bf16_t *out[2] = {bwd ? a.dqkv : a.out_hi, bwd ? a.dqkv_lo : a.out_lo}, *in[4] = {a.qkv_hi, a.qkv_lo, bwd ? a.dout : nullptr, bwd ? a.dout_lo : nullptr};
+        const long ldo = bwd ? a.lddq : a.ldo, ldi[4] = {a.ld, a.ld, a.lddo, a.lddo};
+        auto range = [&](const bf16_t* p, long ld) { return MatRange{(uintptr_t)p, 2, 0, ld, 1, a.rows, (int)W, true, 0}; };
+        for (int i = 0; i < 2; ++i)
+            for (int k = 0; k < 4 && out[i]; ++k)
+                S3D_REQUIRE(!in[k] || (in[k] == out[i] && ldi[k] == ldo && (k & 1) == i) || !ranges_meet(range(out[i], ldo), range(in[k], ldi[k])),
+                            "%s: an output plane overlaps an input plane", who);
+        S3D_REQUIRE(!out[1] || !ranges_meet(range(out[0], ldo), range(out[1], ldo)), "%s: the output planes overlap", who);
     }
     return 0;
 }

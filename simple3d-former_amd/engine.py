@@ -483,6 +483,7 @@ class VoxelEngine:
         for i, v in enumerate((lr, momentum, weight_decay, grad_scale)):
             if v is not None:
                 self._muon_hyper[i:i + 1].fill_(float(v))
+        ops.muon_scale(scale, 1, 1)                # (an unknown rule is refused here, not in the middle of a step)
         muon = (bool(nesterov), int(steps), tuple(float(c) for c in coefficients), scale)
         if muon != self.muon:
             self.capture_epoch += 1                # trainers holding their own captures re-capture (and refuse); this engine's cache is keyed by it

@@ -289,3 +289,32 @@ def test_two_streams_at_once():
                 got[i] = ops.orthogonalize(xs[i])
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_column_blocks_and_row_blocks_of_one_matrix():
+    """Parameters that are blocks of one tensor (their address ranges interleave, their elements do not): the step of separate tensors, bit for bit."""
+    hyper = torch.tensor([0.02, 0.9, 0.1, 1.0], device=DEV)
+    full = [grads(3, 300, 200, seed=s) for s in range(3)]
+    cut = lambda t: [t[:, :120, :64], t[:, :120, 64:200], t[:, 120:300, :], ]
+    cols = lambda t: [t[0, :, :64], t[0, :, 64:70], t[0, :, 70:]]                # count 1
+    for blocks in (cut, cols):
+        apart = [[v.contiguous().clone() for v in blocks(t)] for t in full]
+        both = [t.clone() for t in full]
+        ops.muon_step(*apart, hyper, zero_grad=True)
+        ops.muon_step(*[blocks(t) for t in both], hyper, zero_grad=True)
+        for t, parts in zip(both, apart):
+            for v, w in zip(blocks(t), parts):
+                assert torch.equal(v, w)
+        if blocks is cols:
+            for t, f in zip((both[0], both[2]), (full[0], full[2])):
+                assert torch.equal(t[1:], f[1:])                                 # rows behind the last block are left alone
+
+
+def test_shared_parameters_are_refused():
+    p, g, m = (grads(2, 40, 30, seed=s) for s in range(3))
+    hyper = torch.tensor([0.02, 0.9, 0.1, 1.0], device=DEV)
+    keep = [t.clone() for t in (p, g, m)]
+    for args in (([p, p], [g, g], [m, m]), ([p, p[1]], [g, g[1]], [m, m[1]]), ([p], [g], [g]), ([p[0], p[1]], [g[0], g[1]], [m[0], m[0]])):
+        with pytest.raises(RuntimeError, match='shares memory'):
+            ops.muon_step(*args, hyper)
+    assert all(torch.equal(a, b) for a, b in zip(keep, (p, g, m)))

@@ -112,6 +112,8 @@ def test_refusals():
     for call in (a.adam_step, lambda: a.adam_apply(0, 512)):
         with pytest.raises(RuntimeError, match='set_muon is in effect'):
             call()
+    with pytest.raises(ValueError):
+        a.set_muon(scale='unknown rule')
     a.unset_muon()
     a.adam_step()
     with pytest.raises(ValueError, match='current device'):

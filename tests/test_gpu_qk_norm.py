@@ -270,3 +270,31 @@ def test_rope_table_axes_and_far_positions():
     cos, sin = ops.rope_table(torch.tensor([[1, 2, 3]]), 64)            # 32 pairs: 10 for each axis, two not rotated
     assert cos.shape == (1, 32) and bool((cos[0, 30:] == 1).all()) and bool((sin[0, 30:] == 0).all())
     assert abs(float(sin[0, 10]) - torch.sin(torch.tensor(2.0)).item()) < 1e-7
+
+
+def test_offsets_past_32_bits():
+    """2.3 10^9 elements per plane: the last rows and the last value heads, against the same rows in a tensor of their own."""
+    H, hd, rows = 6, 64, 2_000_003
+    W = 3 * H * hd
+    x = torch.empty(rows, W, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(DEV).manual_seed(5))
+    gain = torch.rand(hd, device=DEV) + 0.5
+    rope = tuple(t.to(DEV) for t in ops.rope_table(torch.arange(1000), hd))
+    pos = (torch.arange(rows, device=DEV) % 1000).int()
+    out, _ = ops.qk_norm_rope_fwd(x, None, H, hd, q_gain=gain, k_gain=gain, rope=rope, pos=pos)
+    dx, _, dq, dk = ops.qk_norm_rope_bwd(out, None, x, None, H, hd, q_gain=gain, k_gain=gain, rope=rope, pos=pos)
+    for s in (slice(0, 700), slice(rows // 2, rows // 2 + 700), slice(rows - 700, rows)):
+        small, _ = ops.qk_norm_rope_fwd(x[s].clone(), None, H, hd, q_gain=gain, k_gain=gain, rope=rope, pos=pos[s].clone())
+        assert torch.equal(out[s], small)
+        back = ops.qk_norm_rope_bwd(small, None, x[s].clone(), None, H, hd, q_gain=gain, k_gain=gain, rope=rope, pos=pos[s].clone())[0]
+        assert torch.equal(dx[s], back)
+    assert bool(torch.isfinite(dq).all()) and bool(torch.isfinite(dk).all())
+
+
+def test_one_gradient_tensor_for_both_gains_is_refused():
+    x = torch.randn(20, 3 * 64, device=DEV).bfloat16()
+    d = torch.zeros(64, device=DEV)
+    with pytest.raises(RuntimeError, match='overlap'):
+        ops.qk_norm_rope_bwd(x.clone(), None, x, None, 1, 64, gain_grads=(d, d))
+    with pytest.raises(RuntimeError, match='overlap'):
+        ops.qk_norm_rope_fwd(x[1:], None, 1, 64, out=(x[:-1], None))
+    assert not bool(d.any())

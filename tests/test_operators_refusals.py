@@ -129,3 +129,59 @@ def test_wrappers_refuse():
         ops.rope_table(torch.zeros(4, 9), 16)
     assert ops.muon_scale('original', 8, 2) == 2.0 and ops.muon_scale('original', 2, 8) == 1.0
     assert ops.muon_scale('match_rms_adamw', 25, 100) == 2.0 and ops.muon_scale(0.5, 3, 3) == 0.5
+
+
+@pytest.mark.parametrize('kw', [
+    dict(out_hi=P + 16), dict(out_hi=P + 576 * 8), dict(qkv_lo=1 << 20, out_hi=1 << 20, out_lo=P), dict(out_lo=2 * P), dict(out_lo=2 * P + 64)])
+def test_qk_norm_forward_refuses_overlapping_planes(lib, kw):
+    """Rows of 576 elements, ten of them: 11520 bytes.  Shifted planes, swapped planes, one plane for both halves of a pair."""
+    f = dict(out_hi=1 << 22)
+    f.update(kw)
+    refused(lib.s3d_qk_norm_rope_fwd(qk(**f), None), lib, 'overlap')
+
+
+@pytest.mark.parametrize('kw', [
+    dict(dk_gain=1 << 23), dict(dk_gain=(1 << 23) + 128), dict(dqkv=(1 << 22) + 1152), dict(dqkv=P + 16), dict(dqkv_lo=(1 << 22) + (1 << 14))])
+def test_qk_norm_backward_refuses_overlapping_tensors(lib, kw):
+    """One gradient tensor for both gains (two workgroups would add to it), shifted planes."""
+    f = dict(out_hi=0, dout=1 << 21, lddo=576, dqkv=(1 << 22) + (1 << 14), lddq=576, dq_gain=1 << 23, dk_gain=1 << 24, partial=P, partial_blocks=1)
+    if 'dqkv' in kw and kw['dqkv'] != P + 16:
+        f['dout'] = 1 << 22
+    f.update(kw)
+    refused(lib.s3d_qk_norm_rope_bwd(qk(**f), None), lib, 'overlap')
+
+
+def items(cls, make, *kws):
+    arr = (cls * len(kws))()
+    for i, kw in enumerate(kws):
+        arr[i] = make(**kw)[0]
+    return arr
+
+
+A = 1 << 20          # one tensor of 2 matrices [10][20]: 1600 bytes
+
+
+@pytest.mark.parametrize('first,second', [
+    (dict(), dict()),                                                           # the same parameter twice
+    (dict(), dict(p=4 * A, g=5 * A)),                                           # one momentum for two parameters
+    (dict(), dict(p=A + 800, g=5 * A, m=6 * A, count=1)),                       # a stack and its second matrix
+    (dict(), dict(p=A + 40, g=5 * A, m=6 * A, count=1)),                        # columns that wrap into the next row
+    (dict(), dict(p=4 * A, g=5 * A, m=A)),                                      # one's momentum, the other's parameter
+    (dict(), dict(p=4 * A, g=A, m=6 * A)),                                      # one's parameter, the other's gradient
+    (dict(g=A), dict(p=4 * A, g=5 * A, m=6 * A)),                               # parameter and gradient of one item
+    (dict(hi=8 * A, lo=8 * A), dict(p=4 * A, g=5 * A, m=6 * A)),                # one plane for both halves
+    (dict(hi=8 * A, lo=A), dict(p=4 * A, g=5 * A, m=6 * A))])                   # a plane in the parameter
+def test_muon_refuses_shared_tensors(lib, first, second):
+    f = [dict(dict(p=A, g=2 * A, m=3 * A), **kw) for kw in (first, second)]
+    refused(lib.s3d_muon_step(items(L.S3dMuonItem, muon, *f), 2, ns(), P, P, 1 << 40, None), lib, 'shares memory')
+
+
+def test_muon_refuses_one_gradient_for_two_parameters_when_it_is_cleared(lib):
+    f = [dict(p=A, g=2 * A, m=3 * A), dict(p=4 * A, g=2 * A, m=6 * A)]
+    refused(lib.s3d_muon_step(items(L.S3dMuonItem, muon, *f), 2, ns(zero_grad=1), P, P, 1 << 40, None), lib, 'shares memory')
+
+
+@pytest.mark.parametrize('second', [dict(x=4 * A), dict(x=4 * A, out=2 * A + 80), dict(x=2 * A + 400, out=5 * A, count=1)])
+def test_orthogonalize_refuses_shared_outputs(lib, second):
+    f = [dict(dict(x=A, out=2 * A), **kw) for kw in ({}, second)]
+    refused(lib.s3d_orthogonalize(items(L.S3dOrthoItem, ortho, *f), 2, ns(), P, 1 << 40, None), lib, 'shares memory')
