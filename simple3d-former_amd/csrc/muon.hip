@@ -101,10 +101,13 @@ __device__ __forceinline__ void split_half(float v, half_t& hi, half_t& lo) {
 // momentum and the direction of the step, elementwise: m' = mu m + (1 - mu) g, u = nesterov ? (1 - mu) g + mu m' : m'
 __device__ __forceinline__ float muon_mix(float g, float m, float mu) { return fmaf(mu, m, (1.f - mu) * g); }
 
-// 8 consecutive elements (n of them inside the row, the rest 0); 16-byte loads where the address allows them
+// 8 consecutive elements (n of them inside the row, the rest 0) in 16-byte accesses, whatever the row's alignment: rows of odd length are
+// not aligned, and global memory takes 16-byte accesses at the element's alignment
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
 __device__ __forceinline__ void load8f(const float* p, int n, float* v) {
-    if (n == 8 && ((uintptr_t)p & 15) == 0) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+    if (n == 8) {
+        const f32x4 a = *reinterpret_cast<const f32x4_any*>(p), b = *reinterpret_cast<const f32x4_any*>(p + 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
     } else {
@@ -113,9 +116,9 @@ __device__ __forceinline__ void load8f(const float* p, int n, float* v) {
     }
 }
 __device__ __forceinline__ void store8f(float* p, int n, const float* v) {
-    if (n == 8 && ((uintptr_t)p & 15) == 0) {
-        *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    if (n == 8) {
+        *reinterpret_cast<f32x4_any*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4_any*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -123,9 +126,9 @@ __device__ __forceinline__ void store8f(float* p, int n, const float* v) {
     }
 }
 __device__ __forceinline__ void load8b(const bf16_t* p, int n, float* v) {
-    if (n == 8 && ((uintptr_t)p & 15) == 0) {
+    if (n == 8) {
         U128 a;
-        a.u = *reinterpret_cast<const u32x4*>(p);
+        a.u = *reinterpret_cast<const u32x4_any*>(p);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = bf2f(a.h[i]);
     } else {
@@ -135,8 +138,8 @@ __device__ __forceinline__ void load8b(const bf16_t* p, int n, float* v) {
 }
 
 __device__ __forceinline__ void store8b(bf16_t* p, int n, const float* v) {
-    if (n == 8 && ((uintptr_t)p & 15) == 0) {
-        *reinterpret_cast<u32x4*>(p) = u32x4{f2bf2(v[0], v[1]), f2bf2(v[2], v[3]), f2bf2(v[4], v[5]), f2bf2(v[6], v[7])};
+    if (n == 8) {
+        *reinterpret_cast<u32x4_any*>(p) = u32x4{f2bf2(v[0], v[1]), f2bf2(v[2], v[3]), f2bf2(v[4], v[5]), f2bf2(v[6], v[7])};
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -618,9 +621,14 @@ int pad_of(long padded64, long padded128) { return padded128 / (128 * 128) >= 12
 bool ns_plan(NsPlan& pl, int n, const int* count, const int* rows, const int* cols) {
     memset(&pl, 0, sizeof(pl));
     pl.t.n = n;
-    long padded[2] = {0, 0};
-    for (int i = 0; i < n; ++i)
+    long padded[2] = {0, 0}, units = 0;
+    for (int i = 0; i < n; ++i) {
         for (int k = 0; k < 2; ++k) padded[k] += (long)count[i] * up(rows[i], 64 << k) * up(cols[i], 64 << k);
+        units += ((long)cols[i] + 7) / 8 * rows[i] * count[i];
+    }
+    // units of one partial sum: one per thread while that leaves few workgroups, else four (sum of squares, us with 256 / 1024 units: a 192-wide block
+    // 5.5 / 7.2, ragged stacks of 309 k units 9.2 / 10.5, 12 x 1536 x 384 11.3 / 8.6)
+    const long chunk = units <= 1024 * 512 ? 256 : 1024;
     pl.pad = pad_of(padded[0], padded[1]);
     long off = 0;
     for (int i = 0; i < n; ++i) {
@@ -628,7 +636,7 @@ bool ns_plan(NsPlan& pl, int n, const int* count, const int* rows, const int* co
         d.count = count[i]; d.rows = rows[i]; d.cols = cols[i];
         d.tall = rows[i] > cols[i];
         d.rp = up(rows[i], pl.pad); d.cp = up(cols[i], pl.pad); d.mp = d.tall ? d.cp : d.rp;
-        const long units = ((long)cols[i] + 7) / 8 * rows[i], chunks = (units + 1023) / 1024;
+        const long chunks = (((long)cols[i] + 7) / 8 * rows[i] + chunk - 1) / chunk;
         d.chunks = (int)(chunks > 512 ? 512 : chunks);
         d.part = pl.parts;
         pl.parts += (long)d.count * d.chunks;

@@ -245,10 +245,18 @@ int lanes_of(int hd) {
     while (g * 16 < hd) g <<= 1;
     return g;
 }
-// rows of one workgroup: one pass of its groups over the heads while there are few rows, about 2048 row ranges (x 3 roles) when there are many
-int rows_per_wg(long rows, int H, int hd) {
+// Rows of one workgroup: one pass of its groups over the heads while there are few rows, about 2048 row ranges (x 3 roles) when there are many.
+// Backward: a workgroup ends by adding its groups' gain gradients through LDS, and every row range is a row of the reduction behind it, so up to four
+// passes as long as 900 workgroups are left.  One / two / four passes, us with the reduction: 1203 ranges of 128-wide heads 23.4 / 17.7 / 16.7,
+// 747 ranges of 64-wide heads 19.6 / 16.6 / 17.3.
+int rows_per_wg(long rows, int H, int hd, bool bwd) {
     const int groups = 256 / lanes_of(hd);
-    const long r = (groups + H - 1) / H, cap = (rows + 2047) / 2048;
+    long r = (groups + H - 1) / H;
+    const long cap = (rows + 2047) / 2048;
+    if (bwd) {
+        const long passes = (rows + r - 1) / r / 300;
+        r *= passes < 1 ? 1 : passes > 4 ? 4 : passes;
+    }
     return (int)(r < cap ? cap : r);
 }
 unsigned inv_of(int b) { return b > 1 ? (unsigned)((1ULL << 32) / (unsigned)b) : 0xffffffffu; }
@@ -256,7 +264,7 @@ unsigned inv_of(int b) { return b > 1 ? (unsigned)((1ULL << 32) / (unsigned)b) :
 template <bool BWD>
 int launch(const S3dQkNormArgs& a, hipStream_t s) {
     QkPlan q;
-    q.rows_per_wg = rows_per_wg(a.rows, a.H, a.hd);
+    q.rows_per_wg = rows_per_wg(a.rows, a.H, a.hd, BWD);
     q.h_inv[0] = inv_of(a.H);
     q.h_inv[1] = inv_of(a.Hkv);
     q.st_inv = inv_of(a.st);
@@ -325,7 +333,7 @@ int check(const S3dQkNormArgs& a, bool bwd) {
 
 int s3d_qk_norm_blocks(long rows, int H, int Hkv, int hd) {
     if (rows <= 0 || H < 1 || Hkv < 1 || hd < 16 || hd > 256) return 0;
-    const int r = rows_per_wg(rows, H, hd);
+    const int r = rows_per_wg(rows, H, hd, true);
     return (int)((rows + r - 1) / r);
 }
 int s3d_launch_qk_norm_fwd(const S3dQkNormArgs& a, hipStream_t s) {
