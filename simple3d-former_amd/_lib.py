@@ -180,11 +180,16 @@ def fill(struct, **kw):
     return struct
 
 
+_current = None
+
+
 def current_stream():
     """The current HIP stream of the current device.  torch.cuda.current_stream() builds a Stream object (2.7 us a call); the raw handle is the
     same value."""
-    import torch
-    raw = getattr(torch._C, '_cuda_getCurrentRawStream', None)
-    if raw is None:
-        return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-    return ctypes.c_void_p(raw(torch.cuda.current_device()))
+    global _current
+    if _current is None:
+        import torch
+        raw = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+        device = torch.cuda.current_device
+        _current = (lambda: raw(device())) if raw is not None else (lambda: torch.cuda.current_stream().cuda_stream)
+    return ctypes.c_void_p(_current())

@@ -307,72 +307,73 @@ __device__ __forceinline__ half8 ns_frag(const unsigned char* tile, int q, int i
         return __builtin_bit_cast(half8, u);
     }
 }
-template <int F>
-struct NsFrags { half8 l[2][F], r[2][F]; };
-// the fragments [from, to) of the 4 F of a stage, and the products [from, to) of its 3 F^2 (pairs: hi hi, hi lo, lo hi) or 2 F^2 (the two halves of
-// a single-plane stage): numbered so that they can be dealt out between the other instructions of a stage
-template <int T, int F, int PL, bool LK, bool RK>
-__device__ __forceinline__ void ns_read(NsFrags<F>& f, const unsigned char* st, int wr, int wc, int lane, int from = 0, int to = 4 * F) {
+template <int FR, int FC>
+struct NsFrags { half8 l[2][FR], r[2][FC]; };
+// the fragments of a stage, and the products [from, to) of its 3 FR FC (pairs: hi hi, hi lo, lo hi) or 2 FR FC (the two halves of a single-plane
+// stage): numbered so that they can be dealt out between the other instructions of a stage
+template <int TR, int TC, int FR, int FC, int PL, bool LK, bool RK>
+__device__ __forceinline__ void ns_read(NsFrags<FR, FC>& f, const unsigned char* st, int wr, int wc, int lane) {
 #pragma unroll
-    for (int e = from; e < to; ++e) {
-        const int q = e / (2 * F), i = (e / 2) % F;
-        if (e & 1) f.r[q][i] = ns_frag<T, PL, RK>(st + T * 128, q, wc + i * 16, lane);
-        else f.l[q][i] = ns_frag<T, PL, LK>(st, q, wr + i * 16, lane);
-    }
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int i = 0; i < (FR > FC ? FR : FC); ++i) {
+            if (i < FR) f.l[q][i] = ns_frag<TR, PL, LK>(st, q, wr + i * 16, lane);
+            if (i < FC) f.r[q][i] = ns_frag<TC, PL, RK>(st + TR * 128, q, wc + i * 16, lane);
+        }
 }
-template <int PL, int F>
-constexpr int ns_products() { return (PL == 2 ? 3 : 2) * F * F; }
-template <int F, int PL>
-__device__ __forceinline__ void ns_mfma(const NsFrags<F>& f, f32x4 (&acc)[F][F], int from = 0, int to = ns_products<PL, F>()) {
+template <int PL, int FR, int FC>
+constexpr int ns_products() { return (PL == 2 ? 3 : 2) * FR * FC; }
+template <int FR, int FC, int PL>
+__device__ __forceinline__ void ns_mfma(const NsFrags<FR, FC>& f, f32x4 (&acc)[FR][FC], int from = 0, int to = ns_products<PL, FR, FC>()) {
 #pragma unroll
     for (int e = from; e < to; ++e) {
-        const int q = e / (F * F), i = e / F % F, j = e % F, ql = PL == 2 ? q == 2 : q, qr = PL == 2 ? q == 1 : q;
+        const int q = e / (FR * FC), i = e / FC % FR, j = e % FC, ql = PL == 2 ? q == 2 : q, qr = PL == 2 ? q == 1 : q;
         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.r[qr][j], f.l[ql][i], acc[i][j], 0, 0, 0);
     }
 }
 
-// acc = sum over k of L(i, k) R(j, k) for a T x T tile by 2 x 2 waves of T/2 x T/2: a ring of
+// acc = sum over k of L(i, k) R(j, k) for a TR x TC tile by 2 x 2 waves of TR/2 x TC/2: a ring of
 // RING stages filled by LDS-DMA; the fragments of the next stage are read while the matrix cores work on this one (a SIMD has
 // two waves: without that the LDS time of a stage adds to its MFMA time).  PL planes (2: hi hi + hi lo + lo hi; stages of 32 k.  1: stages of
 // 64 k).  K is a multiple of 64.  acc[i][j][e] = C[wr + 16 i + (lane & 15)][wc + 16 j + 4 (lane >> 4) + e].
-template <int T, int RING, int PL, bool LK, bool RK>
-__device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& R, int K, unsigned char* smem, f32x4 (&acc)[T / 32][T / 32]) {
-    constexpr int STAGE = 2 * T * 128;                               // bytes: L, R
-    constexpr int PIECES = STAGE / 1024 / 4;                         // 1 KB DMA pieces per wave and stage
-    constexpr int F = T / 32;                                        // 16-row fragments per wave and side
+template <int TR, int TC, int RING, int PL, bool LK, bool RK>
+__device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& R, int K, unsigned char* smem, f32x4 (&acc)[TR / 32][TC / 32]) {
+    constexpr int STAGE = (TR + TC) * 128;                           // bytes: L, R
+    constexpr int PIECES = STAGE / 1024 / 4;                         // 1 KB DMA pieces per wave and stage: wave w brings w PIECES .. of L's and R's
+    constexpr int LEFT = TR / 8, FR = TR / 32, FC = TC / 32;         // L's pieces; 16-row fragments per wave
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    // waves 0, 1 bring L, waves 2, 3 bring R
-    const bool right = wave >= 2;
-    const long step = right ? ns_step<PL, RK>(R) : ns_step<PL, LK>(L);
-    const half_t* src = right ? ns_base<PL, RK>(R) : ns_base<PL, LK>(L);
+    const int left = LEFT - wave * PIECES;                           // this wave's pieces below `left` are L's
+    const long step_l = ns_step<PL, LK>(L), step_r = ns_step<PL, RK>(R);
+    const half_t *src_l = ns_base<PL, LK>(L), *src_r = ns_base<PL, RK>(R);
     unsigned off[PIECES];
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-        const int q = (wave & 1) * PIECES + i;
-        off[i] = right ? ns_source<T, PL, RK>(R, q, lane) : ns_source<T, PL, LK>(L, q, lane);
+        const int q = wave * PIECES + i;
+        off[i] = i < left ? ns_source<TR, PL, LK>(L, q, lane) : ns_source<TC, PL, RK>(R, q - LEFT, lane);
     }
     const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)smem + wave * PIECES * 1024);
     const int KT = K / (PL == 2 ? 32 : 64);
     unsigned slot_in = 0, slot = 0;                                  // in bytes
     auto advance = [](unsigned& s) { s = s == (RING - 1) * STAGE ? 0 : s + STAGE; };
 #pragma unroll
-    for (int i = 0; i < F; ++i)
+    for (int i = 0; i < FR; ++i)
 #pragma unroll
-        for (int j = 0; j < F; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < FC; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int k = 0; k < RING && k < KT; ++k) {
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) ns_dma(src, off[i], lds0 + slot_in + i * 1024);
-        src += step;
+        for (int i = 0; i < PIECES; ++i) ns_dma(i < left ? src_l : src_r, off[i], lds0 + slot_in + i * 1024);
+        src_l += step_l;
+        src_r += step_r;
         advance(slot_in);
     }
-    const int wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
+    const int wr = (wave >> 1) * (TR / 2), wc = (wave & 1) * (TC / 2);
     // stage 0 has landed when at most the later stages' pieces are outstanding
     if (RING <= KT) ns_wait<(RING - 1) * PIECES, false>();
     else ns_wait<0, false>();
     ns_barrier();
-    NsFrags<F> fa, fb;
-    ns_read<T, F, PL, LK, RK>(fa, smem, wr, wc, lane);
-    auto body = [&](int kt, NsFrags<F>& now, NsFrags<F>& next) {
+    NsFrags<FR, FC> fa, fb;
+    ns_read<TR, TC, FR, FC, PL, LK, RK>(fa, smem, wr, wc, lane);
+    auto body = [&](int kt, NsFrags<FR, FC>& now, NsFrags<FR, FC>& next) {
         // this wave holds stage kt in registers (lgkmcnt) and its pieces of stage kt + 1 have landed; behind the barrier that is true of every wave:
         // the slot of stage kt can be refilled, stage kt + 1 can be read (behind the last stage: old data that nobody uses)
         if (RING == 2 || kt + RING > KT) ns_wait<0, true>();
@@ -381,14 +382,15 @@ __device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& 
         const bool more = kt + RING < KT;
         advance(slot);
         // the reads lie under the products (finer interleavings of loads, reads and products measured the same or slower)
-        constexpr int M = ns_products<PL, F>();
+        constexpr int M = ns_products<PL, FR, FC>();
 #pragma unroll
         for (int i = 0; i < PIECES; ++i)
-            if (more) ns_dma(src, off[i], lds0 + slot_in + i * 1024);
-        ns_mfma<F, PL>(now, acc, 0, M / 3);
-        ns_read<T, F, PL, LK, RK>(next, smem + slot, wr, wc, lane);
-        ns_mfma<F, PL>(now, acc, M / 3, M);
-        src += step;
+            if (more) ns_dma(i < left ? src_l : src_r, off[i], lds0 + slot_in + i * 1024);
+        ns_mfma<FR, FC, PL>(now, acc, 0, M / 3);
+        ns_read<TR, TC, FR, FC, PL, LK, RK>(next, smem + slot, wr, wc, lane);
+        ns_mfma<FR, FC, PL>(now, acc, M / 3, M);
+        src_l += step_l;
+        src_r += step_r;
         advance(slot_in);
     };
     for (int kt = 0; kt < KT; kt += 2) {
@@ -428,12 +430,12 @@ __device__ __forceinline__ void ns_product_ksplit(const NsOperand& L, const NsOp
     for (int kt = 0; kt < KT; ++kt) {
         if (kt + RING <= KT) ns_wait<(RING - 1) * PIECES, false>();
         else ns_wait<0, false>();
-        NsFrags<F> f;
-        ns_read<T, F, PL, LK, RK>(f, mine + slot, 0, 0, lane);
+        NsFrags<F, F> f;
+        ns_read<T, T, F, F, PL, LK, RK>(f, mine + slot, 0, 0, lane);
         ns_wait<63, true>();                                         // the slot is in registers: refill it
         if (kt + RING < KT) issue(slot);
         slot = slot == (RING - 1) * STAGE ? 0 : slot + STAGE;
-        ns_mfma<F, PL>(f, acc);
+        ns_mfma<F, F, PL>(f, acc);
     }
     // partial sums: 16 KB per wave in its own ring (read by nobody any more), then rows 16 wave .. + 15 from all four
     f32x4* red = reinterpret_cast<f32x4*>(mine);
@@ -452,13 +454,14 @@ __device__ __forceinline__ void ns_product_ksplit(const NsOperand& L, const NsOp
 }
 
 // How a tile is worked.  TILE_128: 128 x 128, four waves, 66 KB of LDS: two workgroups share a CU, one's start and epilogue lie under the other's
-// products.  TILE_64: 64 x 64, the k range over the four waves: launches with too few 128 x 128 tiles for the CUs.
-enum { TILE_128 = 0, TILE_64 = 1 };
+// products.  TILE_HALF: 128 x 64, 48 KB, three on a CU: half the granularity for half again the LDS traffic per product.  TILE_64: 64 x 64, the
+// k range over the four waves: launches with too few tiles for the CUs.
+enum { TILE_128 = 0, TILE_64 = 1, TILE_HALF = 2 };
 template <int KIND>
 struct NsTile {
-    static constexpr int T = KIND == TILE_64 ? 64 : 128, PITCH = T + 4;
-    static constexpr int SUM_BYTES = T * PITCH * 4;                  // the tile in fp32
-    static constexpr int RING_BYTES = KIND == TILE_64 ? 4 * 2 * 16384 : 2 * 32768;
+    static constexpr int TR = KIND == TILE_64 ? 64 : 128, TC = KIND == TILE_128 ? 128 : 64, PITCH = TC + 4;
+    static constexpr int SUM_BYTES = TR * PITCH * 4;                 // the tile in fp32
+    static constexpr int RING_BYTES = KIND == TILE_64 ? 4 * 2 * 16384 : 2 * (TR + TC) * 128;
     static constexpr int SUM_AT = KIND == TILE_64 ? RING_BYTES : 0;  // over the ring, except where the ring still holds partial sums
     static constexpr int BYTES = KIND == TILE_64 ? RING_BYTES + SUM_BYTES : SUM_BYTES > RING_BYTES ? SUM_BYTES : RING_BYTES;
 };
@@ -475,11 +478,11 @@ __device__ __forceinline__ void ns_store8(half_t* base, bool pair, long r, int c
 
 // f0 .. f2: scale factors of the epilogue; low: what is written are pairs (0: the next product takes one plane)
 template <int KIND, int PL, int EPI>
-__global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : 2) void ns_gemm_kernel(
+__global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_128 ? 2 : 3) void ns_gemm_kernel(
     const NsTable t, const NsPtrs p, half_t* __restrict__ ws, const float* __restrict__ hyper, int which, float f0, float f1, float f2, int low, int zero_grad) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     using Tile = NsTile<KIND>;
-    constexpr int T = Tile::T, PITCH = Tile::PITCH;
+    constexpr int TR = Tile::TR, TC = Tile::TC, PITCH = Tile::PITCH, Q = TR / TC;
     constexpr bool SYM = EPI == EPI_GRAM || EPI == EPI_POLY;
     NsPlace w;
     if (!ns_place(t, w)) return;
@@ -487,20 +490,21 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : 2) void ns_gemm_kernel(
     NsDims d = t.d[0];                                               // (loaded with the counts; the others cost a second round trip)
     if (it) d = t.d[it];
     int ti, tj;
-    if constexpr (SYM) {                                             // lower triangle, row by row: tile = ti (ti + 1) / 2 + tj
-        ti = __builtin_amdgcn_readfirstlane((int)((__builtin_amdgcn_sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f));
-        if (ti * (ti + 1) / 2 > tile) --ti;
-        if ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
-        tj = tile - ti * (ti + 1) / 2;
+    if constexpr (SYM) {                                             // lower triangle, row by row: tile = Q ti (ti + 1) / 2 + tj
+        const int t1 = tile / Q;
+        ti = __builtin_amdgcn_readfirstlane((int)((__builtin_amdgcn_sqrtf(8.f * t1 + 1.f) - 1.f) * 0.5f));
+        if (ti * (ti + 1) / 2 > t1) --ti;
+        if ((ti + 1) * (ti + 2) / 2 <= t1) ++ti;
+        tj = tile - Q * (ti * (ti + 1) / 2);
     } else {
-        const int tc = d.cp / T;
+        const int tc = d.cp / TC;
         ti = tile / tc;
         tj = tile - ti * tc;
     }
     half_t* base = ws + d.ws + mat * d.wsz;
     const half_t* X = base + off_x(d, which);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    float* S = reinterpret_cast<float*>(smem + Tile::SUM_AT);        // the tile, [T][PITCH]
+    float* S = reinterpret_cast<float*>(smem + Tile::SUM_AT);        // the tile, [TR][PITCH]
     auto product = [&](auto lk, auto rk, const NsOperand& L, const NsOperand& R, int K) {
         constexpr bool LK = decltype(lk)::value, RK = decltype(rk)::value;
         if constexpr (KIND == TILE_64) {
@@ -509,30 +513,30 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : 2) void ns_gemm_kernel(
 #pragma unroll
             for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(S + (wave * 16 + (lane & 15)) * PITCH + j * 16 + (lane >> 4) * 4) = acc[j];
         } else {
-            f32x4 acc[T / 32][T / 32];
-            ns_product<T, 2, PL, LK, RK>(L, R, K, smem, acc);
-            float* mine = S + ((wave >> 1) * (T / 2) + (lane & 15)) * PITCH + (wave & 1) * (T / 2) + (lane >> 4) * 4;
+            f32x4 acc[TR / 32][TC / 32];
+            ns_product<TR, TC, 2, PL, LK, RK>(L, R, K, smem, acc);
+            float* mine = S + ((wave >> 1) * (TR / 2) + (lane & 15)) * PITCH + (wave & 1) * (TC / 2) + (lane >> 4) * 4;
             __syncthreads();                                         // every wave has read its last stage: the ring is free
 #pragma unroll
-            for (int i = 0; i < T / 32; ++i)
+            for (int i = 0; i < TR / 32; ++i)
 #pragma unroll
-                for (int j = 0; j < T / 32; ++j) *reinterpret_cast<f32x4*>(mine + i * 16 * PITCH + j * 16) = acc[i][j];
+                for (int j = 0; j < TC / 32; ++j) *reinterpret_cast<f32x4*>(mine + i * 16 * PITCH + j * 16) = acc[i][j];
         }
         __syncthreads();
     };
     const std::false_type rows;                                      // operand stored as rows of k
     const std::true_type kmajor;
     if constexpr (EPI == EPI_GRAM) {
-        const NsOperand L = {X, d.cp, ti * T}, R = {X, d.cp, tj * T};
+        const NsOperand L = {X, d.cp, ti * TR}, R = {X, d.cp, tj * TC};
         if (!d.tall) product(rows, rows, L, R, d.cp);
         else product(kmajor, kmajor, L, R, d.rp);
     } else if constexpr (EPI == EPI_POLY) {
-        const NsOperand L = {base + off_a(d), d.mp, ti * T}, R = {base + off_a(d), d.mp, tj * T};
+        const NsOperand L = {base + off_a(d), d.mp, ti * TR}, R = {base + off_a(d), d.mp, tj * TC};
         product(rows, rows, L, R, d.mp);
     } else {
         const half_t* P = base + off_p(d);
-        if (!d.tall) product(rows, kmajor, NsOperand{P, d.mp, ti * T}, NsOperand{X, d.cp, tj * T}, d.mp);
-        else product(rows, rows, NsOperand{X, d.cp, ti * T}, NsOperand{P, d.mp, tj * T}, d.mp);
+        if (!d.tall) product(rows, kmajor, NsOperand{P, d.mp, ti * TR}, NsOperand{X, d.cp, tj * TC}, d.mp);
+        else product(rows, rows, NsOperand{X, d.cp, ti * TR}, NsOperand{P, d.mp, tj * TC}, d.mp);
     }
     float lr = 0.f, keep = 1.f;
     if constexpr (EPI == EPI_UPDATE) { lr = hyper[0]; keep = 1.f - lr * hyper[2]; lr *= p.scale[it]; }
@@ -540,8 +544,8 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : 2) void ns_gemm_kernel(
     const int ld = SYM ? d.mp : d.cp;
     // rows of the tile, 8 columns per thread
 #pragma unroll 4
-    for (int u = tid; u < T * T / 8; u += 256) {
-        const int lrow = u / (T / 8), lcol = (u % (T / 8)) * 8, r = ti * T + lrow, c = tj * T + lcol;
+    for (int u = tid; u < TR * TC / 8; u += 256) {
+        const int lrow = u / (TC / 8), lcol = (u % (TC / 8)) * 8, r = ti * TR + lrow, c = tj * TC + lcol;
         float* sp = S + lrow * PITCH + lcol;
         float v[8];
         {
@@ -559,7 +563,7 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : 2) void ns_gemm_kernel(
             for (int e = 0; e < 8; ++e) v[e] = fmaf(f1, (float)ah[e] + (float)al[e], v[e]) + (r == c + e ? f2 : 0.f);
         }
         if constexpr (SYM) {
-            if (ti != tj) {                                          // for the mirror image
+            if (tj / Q != ti) {                                         // for the mirror image
                 *reinterpret_cast<f32x4*>(sp) = f32x4{v[0], v[1], v[2], v[3]};
                 *reinterpret_cast<f32x4*>(sp + 4) = f32x4{v[4], v[5], v[6], v[7]};
             }
@@ -592,16 +596,16 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : 2) void ns_gemm_kernel(
         }
     }
     if constexpr (SYM) {
-        if (ti == tj) return;
+        if (tj / Q == ti) return;
         __syncthreads();
         // the mirror image: 4 x 16 (8 columns of the output) x (rows of the output) per wave: one line per 4 lanes, LDS columns two lanes a bank
 #pragma unroll 2
-        for (int u = tid; u < T * T / 8; u += 256) {
-            const int g = u >> 6, lcol8 = (g % (T / 32)) * 4 + (u & 3), lrow = (g / (T / 32)) * 16 + ((u >> 2) & 15);
+        for (int u = tid; u < TR * TC / 8; u += 256) {
+            const int g = u >> 6, lcol8 = (g % (TR / 32)) * 4 + (u & 3), lrow = (g / (TR / 32)) * 16 + ((u >> 2) & 15);
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = S[(lcol8 * 8 + e) * PITCH + lrow];
-            ns_store8(O, low, (long)tj * T + lrow, ti * T + lcol8 * 8, ld, v);
+            ns_store8(O, low, (long)tj * TC + lrow, ti * TR + lcol8 * 8, ld, v);
         }
     }
 }
@@ -649,13 +653,13 @@ bool ns_plan(NsPlan& pl, int n, const int* count, const int* rows, const int* co
     return true;
 }
 enum { TILES_SUMSQ, TILES_LOAD, TILES_SYM, TILES_MULT };
-// workgroups of every stack for one kind of launch on tiles of T; the size of the grid, -1: more than a grid holds
-long ns_grid(NsTable& t, int T, int kind) {
+// workgroups of every stack for one kind of launch on tiles of tr x tc; the size of the grid, -1: more than a grid holds
+long ns_grid(NsTable& t, int kind, int tr = 64, int tc = 64) {
     long at = 0;
     for (int i = 0; i < t.n; ++i) {
         NsDims& d = t.d[i];
-        const long tm = d.mp / T;
-        const long per = kind == TILES_SUMSQ ? d.chunks : kind == TILES_LOAD ? (long)d.rp * d.cp / 2048 : kind == TILES_SYM ? tm * (tm + 1) / 2 : (long)(d.rp / T) * (d.cp / T);
+        const long tm = d.mp / tr;
+        const long per = kind == TILES_SUMSQ ? d.chunks : kind == TILES_LOAD ? (long)d.rp * d.cp / 2048 : kind == TILES_SYM ? tr / tc * (tm * (tm + 1) / 2) : (long)(d.rp / tr) * (d.cp / tc);
         if (per * d.count >= (1L << 28)) return -1;
         d.per = (int)per;
         d.per_inv = per > 1 ? (unsigned)((1ULL << 32) / per) : 0xffffffffu;
@@ -683,28 +687,40 @@ double ns_bounds(double bound, double a, double b, double c, double& pmax) {
 }
 
 struct NsScale { float f0, f1, f2; int low, zero_grad; };
-// Which tile a launch takes: the shorter estimate from times measured on pairs of planes, in us.  A 64 x 64 tile has a CU to itself: 5 for its start
-// and end + 0.9 per 128 k.  A 128 x 128 tile: 5 + 0.85 per 32 k alone on its CU, 5 + 1.15 per 32 k for two that share it.  Measured for the whole
-// chain of five steps, 64 / 128 alone (tiles of 128 in the symmetric products / in P X): 12 x 384^2 (72 / 108) 166 / 236 us, 16 x 384^2 (96 / 144)
-// 251 / 239, 4 x 768^2 (84 / 144) 326 / 354, 12 x 768^2 (252 / 432) 657 / 469, 8 x 384 x 1536 (48 / 288) 277 / 374, 16 x (96 / 576) 493 / 439.
-bool tile_128(const NsTable& t, bool gram, bool sym, int planes) {
-    double n64 = 0., w64 = 0., n128 = 0., w128 = 0., longest = 0.;
+// Which tile a launch takes: the shortest estimate from times measured on pairs of planes, in us: 5 for a tile's start and end, plus per 32 k
+// (n tiles on 256 CUs)                 64 x 64: 0.225, alone on its CU
+//   128 x 128: 0.85 alone, 1.15 for two on a CU             128 x 64: 0.5 alone, 0.75 for two, 1.1 for three.
+// Measured, 64 / 128 for the whole chain of five steps (tiles of 128 in the symmetric products / in P X): 12 x 384^2 (72 / 108) 166 / 236, 16 x 384^2
+// (96 / 144) 251 / 239, 4 x 768^2 (84 / 144) 326 / 354, 12 x 768^2 (252 / 432) 657 / 469, 8 x 384 x 1536 (48 / 288) 277 / 374, 16 x (96 / 576) 493 / 439.
+// 128 x 128 / 128 x 64 for one launch: the four products of twelve 384-wide blocks, Gram 52 / 48, polynomial 27 / 25, P X 63 / 67; 4 x 2048^2, Gram
+// 126 / 121, polynomial 130 / 123, P X 179 / 197; ragged stacks of 192 tiles, P X 15 / 12.
+int tile_kind(const NsTable& t, bool gram, bool sym, int planes) {
+    struct Sum { double n = 0., alone = 0., two = 0., three = 0.; } s64, s128, half;
+    auto add = [](Sum& s, double n, double stages, double alone, double two, double three) {
+        s.n += n;
+        s.two += n * (5. + two * stages);
+        s.three += n * (5. + three * stages);
+        s.alone = fmax(s.alone, 5. + alone * stages);
+    };
     for (int i = 0; i < t.n; ++i) {
         const NsDims& d = t.d[i];
-        const double k = (gram ? (d.tall ? d.rp : d.cp) : d.mp) * (planes == 2 ? 1. : 0.5);
+        const double stages = (gram ? (d.tall ? d.rp : d.cp) : d.mp) * (planes == 2 ? 1. : 0.5) / 32;
         const double m6 = d.mp / 64, m12 = d.mp / 128;
         const double a = d.count * (sym ? m6 * (m6 + 1) / 2 : (double)(d.rp / 64) * (d.cp / 64));
         const double b = d.count * (sym ? m12 * (m12 + 1) / 2 : (double)(d.rp / 128) * (d.cp / 128));
-        n64 += a; w64 += a * (5. + 0.9 * k / 128);
-        n128 += b; w128 += b * (5. + 1.15 * k / 32);
-        if (5. + 0.85 * k / 32 > longest) longest = 5. + 0.85 * k / 32;
+        add(s64, a, stages, 0.225, 0.225, 0.);
+        add(s128, b, stages, 0.85, 1.15, 0.);
+        add(half, 2. * b, stages, 0.5, 0.75, 1.1);
     }
-    const double t64 = ceil(n64 / 256) * w64 / n64, t128 = n128 <= 256 ? longest : ceil(n128 / 512) * w128 / n128;
-    return t128 < t64;
+    const double t64 = ceil(s64.n / 256) * s64.two / s64.n, t128 = s128.n <= 256 ? s128.alone : ceil(s128.n / 512) * s128.two / s128.n;
+    const double th = half.n <= 256 ? half.alone : half.n <= 512 ? fmax(half.alone, half.two / half.n) : ceil(half.n / 768) * half.three / half.n;
+    return th < t64 && th < t128 ? TILE_HALF : t128 < t64 ? TILE_128 : TILE_64;
 }
 template <int KIND, int PL, int EPI>
-int launch_gemm_v(const NsTable& t, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& f, long grid, hipStream_t s) {
+int launch_gemm_v(NsTable& t, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& f, hipStream_t s) {
     using Tile = NsTile<KIND>;
+    const long grid = ns_grid(t, EPI == EPI_GRAM || EPI == EPI_POLY ? TILES_SYM : TILES_MULT, Tile::TR, Tile::TC);
+    S3D_REQUIRE(grid >= 0, "newton_schulz: too many tiles");
     auto k = ns_gemm_kernel<KIND, PL, EPI>;
     if (Tile::BYTES > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, Tile::BYTES);
     hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(256), Tile::BYTES, s, t, p, ws, hyper, which, f.f0, f.f1, f.f2, f.low, f.zero_grad);
@@ -713,19 +729,13 @@ int launch_gemm_v(const NsTable& t, const NsPtrs& p, half_t* ws, const float* hy
 }
 template <int EPI>
 int launch_gemm(NsPlan& pl, int planes, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& f, hipStream_t s) {
-    constexpr bool SYM = EPI == EPI_GRAM || EPI == EPI_POLY;
-    const int kind = SYM ? TILES_SYM : TILES_MULT;
-    long grid;
-    if (pl.pad == 128 && tile_128(pl.t, EPI == EPI_GRAM, SYM, planes)) {
-        grid = ns_grid(pl.t, 128, kind);
-        S3D_REQUIRE(grid >= 0, "newton_schulz: too many tiles");
-        if (planes == 2) return launch_gemm_v<TILE_128, 2, EPI>(pl.t, p, ws, hyper, which, f, grid, s);
-        return launch_gemm_v<TILE_128, 1, EPI>(pl.t, p, ws, hyper, which, f, grid, s);
-    }
-    grid = ns_grid(pl.t, 64, kind);
-    S3D_REQUIRE(grid >= 0, "newton_schulz: too many tiles");
-    if (planes == 2) return launch_gemm_v<TILE_64, 2, EPI>(pl.t, p, ws, hyper, which, f, grid, s);
-    return launch_gemm_v<TILE_64, 1, EPI>(pl.t, p, ws, hyper, which, f, grid, s);
+    const int kind = pl.pad == 128 ? tile_kind(pl.t, EPI == EPI_GRAM, EPI == EPI_GRAM || EPI == EPI_POLY, planes) : TILE_64;
+#define S3D_NS_CASE(k)                                                                                 \
+    if (kind == k) return planes == 2 ? launch_gemm_v<k, 2, EPI>(pl.t, p, ws, hyper, which, f, s)      \
+                                      : launch_gemm_v<k, 1, EPI>(pl.t, p, ws, hyper, which, f, s);
+    S3D_NS_CASE(TILE_128) S3D_NS_CASE(TILE_HALF)
+#undef S3D_NS_CASE
+    return planes == 2 ? launch_gemm_v<TILE_64, 2, EPI>(pl.t, p, ws, hyper, which, f, s) : launch_gemm_v<TILE_64, 1, EPI>(pl.t, p, ws, hyper, which, f, s);
 }
 
 template <int SRC, int LAST>
@@ -733,7 +743,7 @@ int ns_run(NsPlan& pl, const NsPtrs& p, const S3dNsArgs& a, const float* hyper, 
     double* part = reinterpret_cast<double*>(workspace);
     half_t* ws = reinterpret_cast<half_t*>(part + pl.parts);
     NsTable& t = pl.t;
-    long at = ns_grid(t, 64, TILES_SUMSQ);
+    long at = ns_grid(t, TILES_SUMSQ);
     S3D_REQUIRE(at >= 0, "newton_schulz: too many matrices");
     hipLaunchKernelGGL(ns_sumsq_kernel<SRC>, dim3((unsigned)at), dim3(256), 0, s, t, p, hyper, a.nesterov, part);
     S3D_CHECK_LAUNCH_V("newton_schulz_sumsq", SRC);
@@ -743,7 +753,7 @@ int ns_run(NsPlan& pl, const NsPtrs& p, const S3dNsArgs& a, const float* hyper, 
     const int plain_from = LAST == EPI_OUT_BF16 ? a.steps - 2 : a.steps;
     double bound = 1.001;
     float sx = pow2_under(32768., bound);
-    at = ns_grid(t, 64, TILES_LOAD);
+    at = ns_grid(t, TILES_LOAD);
     S3D_REQUIRE(at >= 0, "newton_schulz: too many tiles");
     hipLaunchKernelGGL(ns_load_kernel<SRC>, dim3((unsigned)at), dim3(256), 0, s, t, p, hyper, a.nesterov, part, a.eps, sx, plain_from > 0, ws);
     S3D_CHECK_LAUNCH_V("newton_schulz_load", SRC);

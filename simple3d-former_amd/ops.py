@@ -123,22 +123,20 @@ def cross_entropy(logits, target, weight=None, grad_scale=1.0):
 
 # ---------------------------------------------------------------------------------------------- head norm + position rotation
 def _same_device(who, *tensors):
-    """All tensors on the CURRENT device: the call is enqueued on the current stream of it."""
-    cur = None
-    for t in tensors:
-        if t is None:
-            continue
-        if t.is_cuda and cur is None:
-            cur = torch.cuda.current_device()
-        if not t.is_cuda or t.get_device() != cur:
-            raise ValueError(f'{who}: every tensor must be on the current device, got one on {t.device}')
+    """All tensors on the CURRENT device: the call is enqueued on the current stream of it.  (This and the checks below run before every launch of
+    calls that last a few microseconds: one attribute of a tensor costs 0.1.)"""
+    on = {t.get_device() for t in tensors if t is not None}
+    if on and (min(on) < 0 or on != {torch.cuda.current_device()}):
+        raise ValueError(f'{who}: every tensor must be on the current device, got {sorted({str(t.device) for t in tensors if t is not None})}')
 
 
 def _plane(who, name, t, rows, width):
     """A [rows, width] bf16 plane with contiguous rows; returns its row pitch."""
-    if t.dtype != torch.bfloat16 or t.shape != (rows, width) or t.stride(1) != 1:
-        raise ValueError(f'{who}: {name} must be a bfloat16 [{rows}, {width}] tensor with contiguous rows, got {t.dtype} {tuple(t.shape)} {t.stride()}')
-    return t.stride(0) if rows > 1 else max(t.stride(0), width)
+    if t.dtype == torch.bfloat16 and t.shape == (rows, width):
+        ld, unit = t.stride()
+        if unit == 1:
+            return ld if rows > 1 else max(ld, width)
+    raise ValueError(f'{who}: {name} must be a bfloat16 [{rows}, {width}] tensor with contiguous rows, got {t.dtype} {tuple(t.shape)} {t.stride()}')
 
 
 def _addr(t):
@@ -192,8 +190,7 @@ def _qk_args(who, qkv_hi, qkv_lo, H, hd, Hkv, q_gain, k_gain, rope, pos, st, eps
 
 def _pair_out(who, name, out, like_hi, like_lo, rows, W):
     if out is None:
-        return (torch.empty_like(like_hi, memory_format=torch.contiguous_format),
-                None if like_lo is None else torch.empty_like(like_lo, memory_format=torch.contiguous_format), W)
+        return like_hi.new_empty((rows, W)), None if like_lo is None else like_hi.new_empty((rows, W)), W
     hi, lo = out
     ld = _plane(who, name, hi, rows, W)
     if lo is not None and _plane(who, name + ' (low plane)', lo, rows, W) != ld:
