@@ -476,6 +476,32 @@ __device__ __forceinline__ void ns_store8(half_t* base, bool pair, long r, int c
     if (pair) *reinterpret_cast<half8*>(o + 32) = l;
 }
 
+// the last product's epilogue for n <= 8 elements of a row: the result, or the parameters' step
+template <int EPI>
+__device__ __forceinline__ void ns_finish8(const NsPtrs& p, int it, int mat, int r, int c, int n, float lr, float keep, int zero_grad, float* v) {
+    const long oi = mat * p.os[it] + (long)r * p.old[it] + c;
+    if constexpr (EPI == EPI_OUT_F32) store8f((float*)p.o[it] + oi, n, v);
+    if constexpr (EPI == EPI_OUT_BF16) store8b((bf16_t*)p.o[it] + oi, n, v);
+    if constexpr (EPI == EPI_UPDATE) {
+        float q[8];
+        load8f((const float*)p.o[it] + oi, n, q);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(-lr, v[e], q[e] * keep);
+        store8f((float*)p.o[it] + oi, n, v);
+        if (p.hi[it]) {
+            store8b(p.hi[it] + oi, n, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] -= bf2f(f2bf(v[e]));
+            store8b(p.lo[it] + oi, n, v);
+        }
+        if (zero_grad) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.f;
+            store8f((float*)p.x[it] + mat * p.xs[it] + (long)r * p.xld[it] + c, n, v);
+        }
+    }
+}
+
 // f0 .. f2: scale factors of the epilogue; low: what is written are pairs (0: the next product takes one plane)
 template <int KIND, int PL, int EPI>
 __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_128 ? 2 : 3) void ns_gemm_kernel(
@@ -571,28 +597,7 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_128 ? 2 : 3
         if constexpr (SYM || EPI == EPI_MULT) ns_store8(O, low, r, c, ld, v);
         else {
             const int n = r < d.rows ? (d.cols - c < 8 ? d.cols - c : 8) : 0;
-            if (n <= 0) continue;
-            const long oi = mat * p.os[it] + (long)r * p.old[it] + c;
-            if constexpr (EPI == EPI_OUT_F32) store8f((float*)p.o[it] + oi, n, v);
-            if constexpr (EPI == EPI_OUT_BF16) store8b((bf16_t*)p.o[it] + oi, n, v);
-            if constexpr (EPI == EPI_UPDATE) {
-                float q[8];
-                load8f((const float*)p.o[it] + oi, n, q);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = fmaf(-lr, v[e], q[e] * keep);
-                store8f((float*)p.o[it] + oi, n, v);
-                if (p.hi[it]) {
-                    store8b(p.hi[it] + oi, n, v);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] -= bf2f(f2bf(v[e]));
-                    store8b(p.lo[it] + oi, n, v);
-                }
-                if (zero_grad) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = 0.f;
-                    store8f((float*)p.x[it] + mat * p.xs[it] + (long)r * p.xld[it] + c, n, v);
-                }
-            }
+            if (n > 0) ns_finish8<EPI>(p, it, mat, r, c, n, lr, keep, zero_grad, v);
         }
     }
     if constexpr (SYM) {
@@ -607,6 +612,189 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_128 ? 2 : 3
             for (int e = 0; e < 8; ++e) v[e] = S[(lcol8 * 8 + e) * PITCH + lrow];
             ns_store8(O, low, (long)tj * TC + lrow, ti * TR + lcol8 * 8, ld, v);
         }
+    }
+}
+
+// Polynomial and P X in one launch for smaller sides up to 192: a workgroup forms the 64 rows of P that its 64 x 64 tile needs by itself.  All of A
+// (147 KB as pairs) is on its way to LDS at once; the band of P never leaves it.  Launches of this size last as long as their latencies
+// (start, first load, store, gap: 4 of 5.5 us), so a third of the launches saved is worth the products done m / 64 times over.
+// Eight waves: 2 x 4 over the band's 64 rows and A's m columns, then 2 x 4 over the 64 x 64 tile.
+constexpr int SMALL_M = 192, SMALL_BYTES = SMALL_M * SMALL_M * 4, SMALL_PITCH = 68;
+template <int MT, int PL>
+__device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* X, const NsDims& d, int ti, int tj, float f0, float f1, float f2, unsigned char* smem) {
+    constexpr int SK = PL == 2 ? 32 : 64, KT = MT * 64 / SK, STAGE = MT * 64 * 128, X_STAGE = 64 * 128;      // k of a stage, stages, bytes of A's and X's
+    // X's tile takes the place of the first half of A's stages as soon as they are read, the band of P that of the second half; a 64-wide A leaves
+    // them room behind it
+    constexpr int HALF = (KT + 1) / 2;
+    constexpr unsigned X_AT = MT == 1 ? KT * STAGE : 0, P_AT = MT == 1 ? KT * (STAGE + X_STAGE) : HALF * STAGE;
+    static_assert(MT == 1 || (KT * X_STAGE <= HALF * STAGE && P_AT + KT * X_STAGE <= SMALL_BYTES && KT * STAGE <= SMALL_BYTES), "the tiles fit");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)smem);
+    const int band = (d.tall ? tj : ti) * 64;
+    {
+        const NsOperand op = {A, MT * 64, 0};
+        unsigned off[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) off[i] = ns_source<64, PL, false>(op, wave * MT + i, lane);
+#pragma unroll
+        for (int s = 0; s < KT; ++s)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) ns_dma(A + s * 64, off[i], lds0 + s * STAGE + (wave * MT + i) * 1024);
+    }
+    const int wr = (wave >> 2) * 32, wc = (wave & 3) * MT * 16;
+    half4 ah[2][MT], al[2][MT];                                       // A's own elements under this wave's part of the band
+    f32x4 acc[2][MT];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            ah[i][j] = al[i][j] = half4{0, 0, 0, 0};
+        }
+    auto place = [&](int r, int c, int q) {                           // 4 elements at row r, column c of a stage: byte offset of plane q
+        return r * 128 + (((4 * q + ((c % SK) >> 3)) ^ dma_swz64(r)) << 4) + (c & 7) * 2;
+    };
+    auto square = [&](int s) {
+        const unsigned char* st = smem + s * STAGE;
+        half8 l[2][2], r[2][MT];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) l[q][i] = ns_frag<64, PL, false>(st, q, band + wr + i * 16, lane);
+#pragma unroll
+            for (int j = 0; j < MT; ++j) r[q][j] = ns_frag<64, PL, false>(st, q, wc + j * 16, lane);
+        }
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+            if ((wc + j * 16) / SK == s) {                            // uniform
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int rr = band + wr + i * 16 + (lane & 15), c = wc + j * 16 + (lane >> 4) * 4;
+                    ah[i][j] = *reinterpret_cast<const half4*>(st + place(rr, c, 0));
+                    if constexpr (PL == 2) al[i][j] = *reinterpret_cast<const half4*>(st + place(rr, c, 1));
+                }
+            }
+#pragma unroll
+        for (int q = 0; q < (PL == 2 ? 3 : 2); ++q)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < MT; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r[PL == 2 ? q == 1 : q][j], l[PL == 2 ? q == 2 : q][i], acc[i][j], 0, 0, 0);
+    };
+    // stage s has landed when at most what was issued behind it is outstanding
+    auto first_half = [&](auto self, auto at) {
+        constexpr int S = decltype(at)::value;
+        if constexpr (S < HALF) {
+            ns_wait<(KT - 1 - S) * MT, false>();
+            ns_barrier();
+            square(S);
+            self(self, std::integral_constant<int, S + 1>());
+        }
+    };
+    first_half(first_half, std::integral_constant<int, 0>());
+    ns_wait<63, true>();
+    ns_barrier();
+    {
+        const NsOperand op = {X, d.cp, (d.tall ? ti : tj) * 64};
+        const half_t* src = d.tall ? ns_base<PL, false>(op) : ns_base<PL, true>(op);
+        const long step = d.tall ? ns_step<PL, false>(op) : ns_step<PL, true>(op);
+        const unsigned off = d.tall ? ns_source<64, PL, false>(op, wave, lane) : ns_source<64, PL, true>(op, wave, lane);
+#pragma unroll
+        for (int s = 0; s < KT; ++s) {
+            ns_dma(src, off, lds0 + X_AT + s * X_STAGE + wave * 1024);
+            src += step;
+        }
+    }
+    auto second_half = [&](auto self, auto at) {
+        constexpr int S = decltype(at)::value;
+        if constexpr (S < KT) {
+            ns_wait<KT + (KT - 1 - S) * MT, false>();
+            ns_barrier();
+            square(S);
+            self(self, std::integral_constant<int, S + 1>());
+        }
+    };
+    second_half(second_half, std::integral_constant<int, HALF>());
+    ns_wait<63, true>();
+    ns_barrier();                                                     // A has been read
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            const int r = wr + i * 16 + (lane & 15), c = wc + j * 16 + (lane >> 4) * 4;
+            half4 h, l;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                half_t x, y;
+                split_half(fmaf(f1, (float)ah[i][j][e] + (float)al[i][j][e], acc[i][j][e] * f0) + (band + r == c + e ? f2 : 0.f), x, y);
+                h[e] = x;
+                l[e] = y;
+            }
+            unsigned char* o = smem + P_AT + (c / SK) * X_STAGE;
+            *reinterpret_cast<half4*>(o + place(r, c, 0)) = h;
+            if constexpr (PL == 2) *reinterpret_cast<half4*>(o + place(r, c, 1)) = l;
+        }
+    ns_wait<0, true>();                                               // X's tile has landed, the band is written
+    ns_barrier();
+    f32x4 out[2][1];
+    out[0][0] = out[1][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int o_r = (wave >> 2) * 32, o_c = (wave & 3) * 16;
+    auto last = [&](auto tall) {
+        constexpr bool TALL = decltype(tall)::value;
+#pragma unroll
+        for (int s = 0; s < KT; ++s) {
+            const unsigned char *P = smem + P_AT + s * X_STAGE, *Xs = smem + X_AT + s * X_STAGE;
+            NsFrags<2, 1> f;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) f.l[q][i] = ns_frag<64, PL, false>(TALL ? Xs : P, q, o_r + i * 16, lane);
+                if constexpr (TALL) f.r[q][0] = ns_frag<64, PL, false>(P, q, o_c, lane);
+                else f.r[q][0] = ns_frag<64, PL, true>(Xs, q, o_c, lane);
+            }
+            ns_mfma<2, 1, PL>(f, out);
+        }
+    };
+    if (d.tall) last(std::true_type());
+    else last(std::false_type());
+    ns_wait<63, true>();
+    ns_barrier();                                                     // the operands have been read: the tile in fp32 goes to the front
+    float* S = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) *reinterpret_cast<f32x4*>(S + (o_r + i * 16 + (lane & 15)) * SMALL_PITCH + o_c + (lane >> 4) * 4) = out[i][0];
+    __syncthreads();
+}
+template <int PL, int EPI>
+__global__ __launch_bounds__(512, 1) void ns_small_kernel(
+    const NsTable t, const NsPtrs p, half_t* __restrict__ ws, const float* __restrict__ hyper, int which, float f0, float f1, float f2, float g0, int low,
+    int zero_grad) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    NsPlace w;
+    if (!ns_place(t, w)) return;
+    const int it = w.it, mat = w.mat, tile = w.tile;
+    NsDims d = t.d[0];
+    if (it) d = t.d[it];
+    const int tc = d.cp / 64, ti = tile / tc, tj = tile - ti * tc, tid = threadIdx.x;
+    half_t* base = ws + d.ws + mat * d.wsz;
+    const half_t *A = base + off_a(d), *X = base + off_x(d, which);
+    if (d.mp == 192) ns_small_product<3, PL>(A, X, d, ti, tj, f0, f1, f2, smem);
+    else if (d.mp == 128) ns_small_product<2, PL>(A, X, d, ti, tj, f0, f1, f2, smem);
+    else ns_small_product<1, PL>(A, X, d, ti, tj, f0, f1, f2, smem);
+    float lr = 0.f, keep = 1.f;
+    if constexpr (EPI == EPI_UPDATE) { lr = hyper[0]; keep = 1.f - lr * hyper[2]; lr *= p.scale[it]; }
+    const int lrow = tid >> 3, lcol = (tid & 7) * 8, r = ti * 64 + lrow, c = tj * 64 + lcol;
+    float v[8];
+    {
+        const float* sp = reinterpret_cast<const float*>(smem) + lrow * SMALL_PITCH + lcol;
+        const f32x4 a = *reinterpret_cast<const f32x4*>(sp), b = *reinterpret_cast<const f32x4*>(sp + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { v[e] = a[e] * g0; v[4 + e] = b[e] * g0; }
+    }
+    if constexpr (EPI == EPI_MULT) ns_store8(base + off_x(d, which ^ 1), low, r, c, d.cp, v);
+    else {
+        const int n = r < d.rows ? (d.cols - c < 8 ? d.cols - c : 8) : 0;
+        if (n > 0) ns_finish8<EPI>(p, it, mat, r, c, n, lr, keep, zero_grad, v);
     }
 }
 
@@ -738,6 +926,28 @@ int launch_gemm(NsPlan& pl, int planes, const NsPtrs& p, half_t* ws, const float
     return planes == 2 ? launch_gemm_v<TILE_64, 2, EPI>(pl.t, p, ws, hyper, which, f, s) : launch_gemm_v<TILE_64, 1, EPI>(pl.t, p, ws, hyper, which, f, s);
 }
 
+// Polynomial and P X in one launch?  Sides that fit, tiles of P X on the CUs once over.  Whole call, two launches / one, us: 192 x 192 93 / 76, the
+// four matrices of a 192-wide block 130 / 112.
+bool small_sides(const NsTable& t) {
+    long n = 0;
+    for (int i = 0; i < t.n; ++i) {
+        const NsDims& d = t.d[i];
+        if (d.mp > SMALL_M) return false;
+        n += (long)d.count * (d.rp / 64) * (d.cp / 64);
+    }
+    return n <= 256;
+}
+template <int PL, int EPI>
+int launch_small(NsPlan& pl, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& poly, const NsScale& mult, hipStream_t s) {
+    const long grid = ns_grid(pl.t, TILES_MULT);
+    S3D_REQUIRE(grid >= 0, "newton_schulz: too many tiles");
+    auto k = ns_small_kernel<PL, EPI>;
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_BYTES);
+    hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(512), SMALL_BYTES, s, pl.t, p, ws, hyper, which, poly.f0, poly.f1, poly.f2, mult.f0, mult.low, mult.zero_grad);
+    S3D_CHECK_LAUNCH_V("newton_schulz_small", PL * 10 + EPI);
+    return 0;
+}
+
 template <int SRC, int LAST>
 int ns_run(NsPlan& pl, const NsPtrs& p, const S3dNsArgs& a, const float* hyper, void* workspace, hipStream_t s) {
     double* part = reinterpret_cast<double*>(workspace);
@@ -751,6 +961,7 @@ int ns_run(NsPlan& pl, const NsPtrs& p, const S3dNsArgs& a, const float* hyper, 
     // per step up to the result: 2 * 2^-12 (a^2 + a) = 0.7 % of its 2-norm at the very most.  Measured beside the 0.17 % of the result's own
     // rounding: 0.05 - 0.1 % for noise and for a few strong directions, 0.3 % for a matrix of rank one; a third such step would triple it.
     const int plain_from = LAST == EPI_OUT_BF16 ? a.steps - 2 : a.steps;
+    const bool small = small_sides(t);
     double bound = 1.001;
     float sx = pow2_under(32768., bound);
     at = ns_grid(t, TILES_LOAD);
@@ -763,9 +974,16 @@ int ns_run(NsPlan& pl, const NsPtrs& p, const S3dNsArgs& a, const float* hyper, 
         const float sa = pow2_under(32768., bound * bound), sp = pow2_under(32768., pmax), sn = pow2_under(32768., next);
         const int planes = k >= plain_from ? 1 : 2, low = planes == 2, low_x = k + 1 < plain_from;
         if (int rc = launch_gemm<EPI_GRAM>(pl, planes, p, ws, hyper, k & 1, {sa / (sx * sx), 0.f, 0.f, low, 0}, s)) return rc;
-        if (int rc = launch_gemm<EPI_POLY>(pl, planes, p, ws, hyper, k & 1, {a.c * sp / (sa * sa), a.b * sp / sa, a.a * sp, low, 0}, s)) return rc;
-        const int rc = k + 1 < a.steps ? launch_gemm<EPI_MULT>(pl, planes, p, ws, hyper, k & 1, {sn / (sp * sx), 0.f, 0.f, low_x, 0}, s)
-                                       : launch_gemm<LAST>(pl, planes, p, ws, hyper, k & 1, {1.f / (sp * sx), 0.f, 0.f, 0, a.zero_grad}, s);
+        const NsScale poly = {a.c * sp / (sa * sa), a.b * sp / sa, a.a * sp, low, 0}, mult = {sn / (sp * sx), 0.f, 0.f, low_x, 0}, last = {1.f / (sp * sx), 0.f, 0.f, 0, a.zero_grad};
+        const bool end = k + 1 == a.steps;
+        int rc;
+        if (small) {
+            if (planes == 2) rc = end ? launch_small<2, LAST>(pl, p, ws, hyper, k & 1, poly, last, s) : launch_small<2, EPI_MULT>(pl, p, ws, hyper, k & 1, poly, mult, s);
+            else rc = end ? launch_small<1, LAST>(pl, p, ws, hyper, k & 1, poly, last, s) : launch_small<1, EPI_MULT>(pl, p, ws, hyper, k & 1, poly, mult, s);
+        } else {
+            rc = launch_gemm<EPI_POLY>(pl, planes, p, ws, hyper, k & 1, poly, s);
+            if (!rc) rc = end ? launch_gemm<LAST>(pl, planes, p, ws, hyper, k & 1, last, s) : launch_gemm<EPI_MULT>(pl, planes, p, ws, hyper, k & 1, mult, s);
+        }
         if (rc) return rc;
         sx = sn;
         bound = next;

@@ -46,7 +46,7 @@ def grads(L, r, c, seed=0, dtype=torch.float32):
 
 
 SHAPES = [(1, 1, 1), (2, 1, 7), (2, 9, 1), (3, 5, 3), (1, 16, 16), (1, 64, 64), (2, 65, 64), (1, 63, 130), (2, 130, 63), (1, 192, 192), (2, 192, 576), (2, 576, 192),
-          (1, 387, 1000), (1, 1000, 387), (3, 384, 384), (1, 768, 768), (1, 2, 5000), (1, 1031, 129), (5, 128, 256), (1, 129, 257),
+          (1, 387, 1000), (1, 1000, 387), (3, 384, 384), (1, 768, 768), (1, 2, 5000), (1, 1031, 129), (5, 128, 256), (1, 129, 257), (2, 500, 100), (3, 90, 100),
           # enough tiles for the large ones: wide, tall, square, padded
           (12, 384, 1536), (12, 1536, 384), (2, 1536, 1530), (2, 1500, 1600), (9, 700, 640), (30, 250, 384)]
 
@@ -318,3 +318,20 @@ def test_shared_parameters_are_refused():
         with pytest.raises(RuntimeError, match='shares memory'):
             ops.muon_step(*args, hyper)
     assert all(torch.equal(a, b) for a, b in zip(keep, (p, g, m)))
+
+
+@pytest.mark.parametrize('shapes', [[(1, 192, 192)], [(2, 64, 300), (1, 300, 60)], [(3, 128, 200), (2, 210, 100)], [(1, 150, 700), (1, 700, 190), (2, 30, 90)]])
+@pytest.mark.parametrize('zero', [False, True])
+def test_muon_step_over_small_sides(shapes, zero):
+    """smaller sides of one, two and three tiles, wide and tall, apart and mixed: polynomial and product in one launch"""
+    g = torch.Generator().manual_seed(1)
+    p, gr, m = [[(torch.randn(*s, generator=g) * k).to(DEV) for s in shapes] for k in (0.02, 1e-3, 1e-3)]
+    planes = [tuple(torch.zeros(*s, dtype=torch.bfloat16, device=DEV) for _ in range(2)) for s in shapes]
+    hyper = torch.tensor([2e-3, 0.95, 0.1, 1.0], device=DEV)
+    p0, m0, g0 = [t.clone() for t in p], [t.clone() for t in m], [t.clone() for t in gr]
+    ops.muon_step(p, gr, m, hyper, planes=planes, zero_grad=zero)
+    for i, s in enumerate(shapes):
+        check_muon(p0[i], g0[i], m0[i], p[i], m[i], hyper, True, ops.muon_scale('original', *s[1:]))
+        hi = p[i].bfloat16()
+        assert torch.equal(planes[i][0], hi) and torch.equal(planes[i][1], (p[i] - hi.float()).bfloat16())
+        assert torch.equal(gr[i], torch.zeros_like(gr[i]) if zero else g0[i])
