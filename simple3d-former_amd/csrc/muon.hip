@@ -231,12 +231,14 @@ __global__ __launch_bounds__(256) void ns_load_kernel(const NsTable t, const NsP
         __syncthreads();
     }
     const double nrm = sqrt(red[0]);
-    const float inv = (float)(1. / (nrm > (double)eps ? nrm : (nrm == nrm ? (double)eps : nrm)));
+    // 1 / |U| in two parts: rounded to fp32 it moves all singular values together
+    const double exact = (double)sx / (nrm > (double)eps ? nrm : (nrm == nrm ? (double)eps : nrm));
+    const float inv = (float)exact, inv_low = (float)(exact - (double)inv);
     half8 h, l;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         half_t a, b;
-        split_half(i < n ? u[i] * inv * sx : 0.f, a, b);
+        split_half(i < n ? fmaf(u[i], inv, u[i] * inv_low) : 0.f, a, b);
         h[i] = a;
         l[i] = b;
     }
@@ -289,55 +291,90 @@ __device__ __forceinline__ void ns_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// fragment q of rows / columns i16 .. + 15: q = plane (pairs), or which half of the stage's 64 k (single planes)
+// A lane's LDS address of the fragments whose rows / columns begin at w0 (a multiple of 32, of 16 for a single one), of an operand's tile at `tile`
+// (a multiple of 512); fragment (q, i), rows / columns w0 + 16 i .. + 15, is a constant away: q = plane (pairs), or which half of the stage's 64 k.  Both
+// swizzles depend on the lane alone, so that one register per operand is kept instead of one per fragment.
 template <int T, int PL, bool KM>
-__device__ __forceinline__ half8 ns_frag(const unsigned char* tile, int q, int i16, int lane) {
+__device__ __forceinline__ unsigned ns_lane(const unsigned char* tile, int w0, int lane) {
     if constexpr (!KM) {
-        const int r = i16 + (lane & 15);
-        return *reinterpret_cast<const half8*>(tile + r * 128 + (((q * 4 + (lane >> 4)) ^ dma_swz64(r)) << 4));
+        const int r = w0 + (lane & 15);
+        return (unsigned)(uintptr_t)tile + r * 128 + (((lane >> 4) ^ dma_swz64(r)) << 4);
+    } else return kmajor_addr<PL * T>(tile, PL == 2 ? (w0 >> 5) * 64 + (w0 & 31) : w0, (lane >> 4) * 8, lane);
+}
+template <int T, int PL, bool KM>
+__device__ __forceinline__ half8 ns_frag(unsigned at, int q, int i) {
+    if constexpr (!KM) {
+        typedef __attribute__((address_space(3))) half8 lds_half8;
+        return *(const lds_half8*)(uintptr_t)((at ^ (q * 64)) + i * 2048);
     } else {
         typedef __attribute__((ext_vector_type(4))) short short4v;
         typedef __attribute__((address_space(3))) short4v lds_short4;
-        constexpr int W = PL * T;
+        constexpr int ROW = PL * T * 2;                                              // bytes
         struct { short4v a, b; } u;
-        const unsigned ad = PL == 2 ? kmajor_addr<W>(tile, (i16 >> 5) * 64 + q * 32 + (i16 & 31), (lane >> 4) * 8, lane)
-                                    : kmajor_addr<W>(tile, i16, q * 32 + (lane >> 4) * 8, lane);
+        const unsigned ad = PL == 2 ? at ^ ((i >> 1) * 128 + q * 64 + (i & 1) * 32) : (at ^ (i * 32)) + q * 32 * ROW;
         u.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)ad);
-        u.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)(ad + 4 * W * 2));
+        u.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)(ad + 4 * ROW));
         return __builtin_bit_cast(half8, u);
     }
 }
 template <int FR, int FC>
 struct NsFrags { half8 l[2][FR], r[2][FC]; };
-// the fragments of a stage, and the products [from, to) of its 3 FR FC (pairs: hi hi, hi lo, lo hi) or 2 FR FC (the two halves of a single-plane
+// the fragments of a stage, and the products [from, to) of its 3 FR FC (pairs: hi lo, lo hi, hi hi) or 2 FR FC (the two halves of a single-plane
 // stage): numbered so that they can be dealt out between the other instructions of a stage
-template <int TR, int TC, int FR, int FC, int PL, bool LK, bool RK>
-__device__ __forceinline__ void ns_read(NsFrags<FR, FC>& f, const unsigned char* st, int wr, int wc, int lane) {
+template <int T, int F, int PL, bool KM>
+__device__ __forceinline__ void ns_read(half8 (&f)[2][F], unsigned at) {
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int i = 0; i < (FR > FC ? FR : FC); ++i) {
-            if (i < FR) f.l[q][i] = ns_frag<TR, PL, LK>(st, q, wr + i * 16, lane);
-            if (i < FC) f.r[q][i] = ns_frag<TC, PL, RK>(st + TR * 128, q, wc + i * 16, lane);
-        }
+        for (int i = 0; i < F; ++i) f[q][i] = ns_frag<T, PL, KM>(at, q, i);
 }
 template <int PL, int FR, int FC>
 constexpr int ns_products() { return (PL == 2 ? 3 : 2) * FR * FC; }
-template <int FR, int FC, int PL>
-__device__ __forceinline__ void ns_mfma(const NsFrags<FR, FC>& f, f32x4 (&acc)[FR][FC], int from = 0, int to = ns_products<PL, FR, FC>()) {
+// Sums of a tile.  The matrix cores' accumulation rounds towards zero at the size of what is there, so one running sum of three products per 32 k is
+// off to one side, for all singular values together (results of orthogonalize 1.1e-6 .. 2.3e-6 off in the 2-norm; 0.5e-6 .. 0.7e-6 with these and the shift of A below).
+// SPLIT (the short sums of a wave that has a part of k): hi hi in one sum, the two products 2^11 smaller in another.  Else: two stages begin at zero,
+// small products first, and are added to a total that rounds to nearest.  (Single planes: one sum.)
+template <int FR, int FC, int PL, bool SPLIT>
+struct NsSums {
+    f32x4 sum[FR][FC], more[FR][FC];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < FR; ++i)
+#pragma unroll
+            for (int j = 0; j < FC; ++j) sum[i][j] = more[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ void flush() {
+        if constexpr (PL == 2 && !SPLIT) {
+#pragma unroll
+            for (int i = 0; i < FR; ++i)
+#pragma unroll
+                for (int j = 0; j < FC; ++j) more[i][j] += sum[i][j];
+        }
+    }
+    __device__ __forceinline__ f32x4 get(int i, int j) const {
+        if constexpr (PL == 1) return sum[i][j];
+        else if constexpr (SPLIT) return sum[i][j] + more[i][j];
+        else return more[i][j];
+    }
+};
+// FIRST: the first of two stages
+template <bool FIRST, int FR, int FC, int PL, bool SPLIT>
+__device__ __forceinline__ void ns_mfma(const NsFrags<FR, FC>& f, NsSums<FR, FC, PL, SPLIT>& acc, int from = 0, int to = ns_products<PL, FR, FC>()) {
 #pragma unroll
     for (int e = from; e < to; ++e) {
-        const int q = e / (FR * FC), i = e / FC % FR, j = e % FC, ql = PL == 2 ? q == 2 : q, qr = PL == 2 ? q == 1 : q;
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.r[qr][j], f.l[ql][i], acc[i][j], 0, 0, 0);
+        const int q = e / (FR * FC), i = e / FC % FR, j = e % FC, ql = PL == 2 ? q == 1 : q, qr = PL == 2 ? q == 0 : q;
+        f32x4& a = SPLIT && PL == 2 && q < 2 ? acc.more[i][j] : acc.sum[i][j];
+        const f32x4 c = !SPLIT && FIRST && PL == 2 && q == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : a;
+        a = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.r[qr][j], f.l[ql][i], c, 0, 0, 0);
     }
 }
 
 // acc = sum over k of L(i, k) R(j, k) for a TR x TC tile by 2 x 2 waves of TR/2 x TC/2: a ring of
 // RING stages filled by LDS-DMA; the fragments of the next stage are read while the matrix cores work on this one (a SIMD has
-// two waves: without that the LDS time of a stage adds to its MFMA time).  PL planes (2: hi hi + hi lo + lo hi; stages of 32 k.  1: stages of
-// 64 k).  K is a multiple of 64.  acc[i][j][e] = C[wr + 16 i + (lane & 15)][wc + 16 j + 4 (lane >> 4) + e].
+// two waves: without that the LDS time of a stage adds to its MFMA time).  PL planes (2: hi lo + lo hi + hi hi; stages of 32 k.  1: stages of
+// 64 k).  K is a multiple of 64.  acc.get(i, j)[e] = C[wr + 16 i + (lane & 15)][wc + 16 j + 4 (lane >> 4) + e].
 template <int TR, int TC, int RING, int PL, bool LK, bool RK>
-__device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& R, int K, unsigned char* smem, f32x4 (&acc)[TR / 32][TC / 32]) {
+__device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& R, int K, unsigned char* smem, NsSums<TR / 32, TC / 32, PL, false>& acc) {
     constexpr int STAGE = (TR + TC) * 128;                           // bytes: L, R
     constexpr int PIECES = STAGE / 1024 / 4;                         // 1 KB DMA pieces per wave and stage: wave w brings w PIECES .. of L's and R's
     constexpr int LEFT = TR / 8, FR = TR / 32, FC = TC / 32;         // L's pieces; 16-row fragments per wave
@@ -355,10 +392,7 @@ __device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& 
     const int KT = K / (PL == 2 ? 32 : 64);
     unsigned slot_in = 0, slot = 0;                                  // in bytes
     auto advance = [](unsigned& s) { s = s == (RING - 1) * STAGE ? 0 : s + STAGE; };
-#pragma unroll
-    for (int i = 0; i < FR; ++i)
-#pragma unroll
-        for (int j = 0; j < FC; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    acc.clear();
     for (int k = 0; k < RING && k < KT; ++k) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) ns_dma(i < left ? src_l : src_r, off[i], lds0 + slot_in + i * 1024);
@@ -372,8 +406,11 @@ __device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& 
     else ns_wait<0, false>();
     ns_barrier();
     NsFrags<FR, FC> fa, fb;
-    ns_read<TR, TC, FR, FC, PL, LK, RK>(fa, smem, wr, wc, lane);
-    auto body = [&](int kt, NsFrags<FR, FC>& now, NsFrags<FR, FC>& next) {
+    const unsigned lane_l = ns_lane<TR, PL, LK>(smem, wr, lane), lane_r = ns_lane<TC, PL, RK>(smem + TR * 128, wc, lane);
+    ns_read<TR, FR, PL, LK>(fa.l, lane_l);
+    ns_read<TC, FC, PL, RK>(fa.r, lane_r);
+    auto body = [&](auto first, int kt, NsFrags<FR, FC>& now, NsFrags<FR, FC>& next) {
+        constexpr bool FIRST = decltype(first)::value;
         // this wave holds stage kt in registers (lgkmcnt) and its pieces of stage kt + 1 have landed; behind the barrier that is true of every wave:
         // the slot of stage kt can be refilled, stage kt + 1 can be read (behind the last stage: old data that nobody uses)
         if (RING == 2 || kt + RING > KT) ns_wait<0, true>();
@@ -386,16 +423,19 @@ __device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& 
 #pragma unroll
         for (int i = 0; i < PIECES; ++i)
             if (more) ns_dma(i < left ? src_l : src_r, off[i], lds0 + slot_in + i * 1024);
-        ns_mfma<FR, FC, PL>(now, acc, 0, M / 3);
-        ns_read<TR, TC, FR, FC, PL, LK, RK>(next, smem + slot, wr, wc, lane);
-        ns_mfma<FR, FC, PL>(now, acc, M / 3, M);
+        ns_mfma<FIRST>(now, acc, 0, M / 3);
+        ns_read<TR, FR, PL, LK>(next.l, lane_l + slot);
+        ns_mfma<FIRST>(now, acc, M / 3, 2 * M / 3);
+        ns_read<TC, FC, PL, RK>(next.r, lane_r + slot);              // (lo of either side is done: all at once are 32 registers more)
+        ns_mfma<FIRST>(now, acc, 2 * M / 3, M);
         src_l += step_l;
         src_r += step_r;
         advance(slot_in);
     };
     for (int kt = 0; kt < KT; kt += 2) {
-        body(kt, fa, fb);
-        if (kt + 1 < KT) body(kt + 1, fb, fa);
+        body(std::true_type(), kt, fa, fb);
+        if (kt + 1 < KT) body(std::false_type(), kt + 1, fb, fa);
+        acc.flush();
     }
 }
 
@@ -421,28 +461,27 @@ __device__ __forceinline__ void ns_product_ksplit(const NsOperand& L, const NsOp
         src_l += 4 * step_l;
         src_r += 4 * step_r;
     };
-    f32x4 acc[F][F];
-#pragma unroll
-    for (int i = 0; i < F; ++i)
-#pragma unroll
-        for (int j = 0; j < F; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    NsSums<F, F, PL, true> acc;
+    acc.clear();
+    const unsigned lane_l = ns_lane<T, PL, LK>(mine, 0, lane), lane_r = ns_lane<T, PL, RK>(mine + T * 128, 0, lane);
     for (int k = 0; k < RING && k < KT; ++k) issue(k * STAGE);
     for (int kt = 0; kt < KT; ++kt) {
         if (kt + RING <= KT) ns_wait<(RING - 1) * PIECES, false>();
         else ns_wait<0, false>();
         NsFrags<F, F> f;
-        ns_read<T, T, F, F, PL, LK, RK>(f, mine + slot, 0, 0, lane);
+        ns_read<T, F, PL, LK>(f.l, lane_l + slot);
+        ns_read<T, F, PL, RK>(f.r, lane_r + slot);
         ns_wait<63, true>();                                         // the slot is in registers: refill it
         if (kt + RING < KT) issue(slot);
         slot = slot == (RING - 1) * STAGE ? 0 : slot + STAGE;
-        ns_mfma<F, F, PL>(f, acc);
+        ns_mfma<false>(f, acc);
     }
     // partial sums: 16 KB per wave in its own ring (read by nobody any more), then rows 16 wave .. + 15 from all four
     f32x4* red = reinterpret_cast<f32x4*>(mine);
 #pragma unroll
     for (int i = 0; i < F; ++i)
 #pragma unroll
-        for (int j = 0; j < F; ++j) red[(i * F + j) * 64 + lane] = acc[i][j];
+        for (int j = 0; j < F; ++j) red[(i * F + j) * 64 + lane] = acc.get(i, j);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < F; ++j) {
@@ -502,11 +541,14 @@ __device__ __forceinline__ void ns_finish8(const NsPtrs& p, int it, int mat, int
     }
 }
 
-// f0 .. f2: scale factors of the epilogue; low: what is written are pairs (0: the next product takes one plane)
+// f0 .. f2: scale factors of the epilogue (below); low: what is written are pairs (0: the next product takes one plane)
+struct NsScale { float f0, f1, f2; int low, zero_grad; };
+__device__ __forceinline__ float ns_poly(const NsScale& f, float square, float a, bool diagonal) { return fmaf(f.f1, a, f.f0 * square) + (diagonal ? f.f2 : 0.f); }
+
 template <int KIND, int PL, int EPI>
 __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_128 ? 2 : 3) void ns_gemm_kernel(
-    const NsTable t, const NsPtrs p, half_t* __restrict__ ws, const float* __restrict__ hyper, int which, float f0, float f1, float f2, int low, int zero_grad) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const NsTable t, const NsPtrs p, half_t* __restrict__ ws, const float* __restrict__ hyper, int which, const NsScale f) {
+    extern __shared__ __attribute__((aligned(512))) unsigned char smem[];
     using Tile = NsTile<KIND>;
     constexpr int TR = Tile::TR, TC = Tile::TC, PITCH = Tile::PITCH, Q = TR / TC;
     constexpr bool SYM = EPI == EPI_GRAM || EPI == EPI_POLY;
@@ -539,14 +581,14 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_128 ? 2 : 3
 #pragma unroll
             for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(S + (wave * 16 + (lane & 15)) * PITCH + j * 16 + (lane >> 4) * 4) = acc[j];
         } else {
-            f32x4 acc[TR / 32][TC / 32];
+            NsSums<TR / 32, TC / 32, PL, false> acc;
             ns_product<TR, TC, 2, PL, LK, RK>(L, R, K, smem, acc);
             float* mine = S + ((wave >> 1) * (TR / 2) + (lane & 15)) * PITCH + (wave & 1) * (TC / 2) + (lane >> 4) * 4;
             __syncthreads();                                         // every wave has read its last stage: the ring is free
 #pragma unroll
             for (int i = 0; i < TR / 32; ++i)
 #pragma unroll
-                for (int j = 0; j < TC / 32; ++j) *reinterpret_cast<f32x4*>(mine + i * 16 * PITCH + j * 16) = acc[i][j];
+                for (int j = 0; j < TC / 32; ++j) *reinterpret_cast<f32x4*>(mine + i * 16 * PITCH + j * 16) = acc.get(i, j);
         }
         __syncthreads();
     };
@@ -577,16 +619,23 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_128 ? 2 : 3
         {
             const f32x4 a = *reinterpret_cast<const f32x4*>(sp), b = *reinterpret_cast<const f32x4*>(sp + 4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { v[e] = a[e] * f0; v[4 + e] = b[e] * f0; }
+            for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
         }
-        // GRAM: f0 = sA / sX^2.  POLY: (a I + b A + c A^2) sP: f0 = c sP / sA^2, f1 = b sP / sA, f2 = a sP.  MULT: f0 = sX' / (sP sX).  Last: 1 / (sP sX)
+        // GRAM: f0 = sA / sX^2, f2 = -shift sA.  POLY: f0 = c sP / sA^2, f1 = b' sP / sA, f2 = a' sP.  MULT: f0 = sX' / (sP sX).  Last: 1 / (sP sX)
         if constexpr (EPI == EPI_POLY) {
             const half_t* A = base + off_a(d) + ns_at(PL == 2, r, c, d.mp);
             const half8 ah = *reinterpret_cast<const half8*>(A);
             half8 al = {0, 0, 0, 0, 0, 0, 0, 0};
             if constexpr (PL == 2) al = *reinterpret_cast<const half8*>(A + 32);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = fmaf(f1, (float)ah[e] + (float)al[e], v[e]) + (r == c + e ? f2 : 0.f);
+            for (int e = 0; e < 8; ++e) v[e] = ns_poly(f, v[e], (float)ah[e] + (float)al[e], r == c + e);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= f.f0;
+        }
+        if constexpr (EPI == EPI_GRAM) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += r == c + e ? f.f2 : 0.f;
         }
         if constexpr (SYM) {
             if (tj / Q != ti) {                                         // for the mirror image
@@ -594,10 +643,10 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_128 ? 2 : 3
                 *reinterpret_cast<f32x4*>(sp + 4) = f32x4{v[4], v[5], v[6], v[7]};
             }
         }
-        if constexpr (SYM || EPI == EPI_MULT) ns_store8(O, low, r, c, ld, v);
+        if constexpr (SYM || EPI == EPI_MULT) ns_store8(O, f.low, r, c, ld, v);
         else {
             const int n = r < d.rows ? (d.cols - c < 8 ? d.cols - c : 8) : 0;
-            if (n > 0) ns_finish8<EPI>(p, it, mat, r, c, n, lr, keep, zero_grad, v);
+            if (n > 0) ns_finish8<EPI>(p, it, mat, r, c, n, lr, keep, f.zero_grad, v);
         }
     }
     if constexpr (SYM) {
@@ -610,7 +659,7 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_128 ? 2 : 3
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = S[(lcol8 * 8 + e) * PITCH + lrow];
-            ns_store8(O, low, (long)tj * TC + lrow, ti * TR + lcol8 * 8, ld, v);
+            ns_store8(O, f.low, (long)tj * TC + lrow, ti * TR + lcol8 * 8, ld, v);
         }
     }
 }
@@ -621,7 +670,7 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_128 ? 2 : 3
 // Eight waves: 2 x 4 over the band's 64 rows and A's m columns, then 2 x 4 over the 64 x 64 tile.
 constexpr int SMALL_M = 192, SMALL_BYTES = SMALL_M * SMALL_M * 4, SMALL_PITCH = 68;
 template <int MT, int PL>
-__device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* X, const NsDims& d, int ti, int tj, float f0, float f1, float f2, unsigned char* smem) {
+__device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* X, const NsDims& d, int ti, int tj, const NsScale& poly, unsigned char* smem) {
     constexpr int SK = PL == 2 ? 32 : 64, KT = MT * 64 / SK, STAGE = MT * 64 * 128, X_STAGE = 64 * 128;      // k of a stage, stages, bytes of A's and X's
     // X's tile takes the place of the first half of A's stages as soon as they are read, the band of P that of the second half; a 64-wide A leaves
     // them room behind it
@@ -643,27 +692,21 @@ __device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* 
     }
     const int wr = (wave >> 2) * 32, wc = (wave & 3) * MT * 16;
     half4 ah[2][MT], al[2][MT];                                       // A's own elements under this wave's part of the band
-    f32x4 acc[2][MT];
+    NsSums<2, MT, PL, true> acc;
+    acc.clear();
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < MT; ++j) {
-            acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            ah[i][j] = al[i][j] = half4{0, 0, 0, 0};
-        }
+        for (int j = 0; j < MT; ++j) ah[i][j] = al[i][j] = half4{0, 0, 0, 0};
     auto place = [&](int r, int c, int q) {                           // 4 elements at row r, column c of a stage: byte offset of plane q
         return r * 128 + (((4 * q + ((c % SK) >> 3)) ^ dma_swz64(r)) << 4) + (c & 7) * 2;
     };
+    const unsigned lane_l = ns_lane<64, PL, false>(smem, band + wr, lane), lane_r = ns_lane<64, PL, false>(smem, wc, lane);
     auto square = [&](int s) {
         const unsigned char* st = smem + s * STAGE;
-        half8 l[2][2], r[2][MT];
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) l[q][i] = ns_frag<64, PL, false>(st, q, band + wr + i * 16, lane);
-#pragma unroll
-            for (int j = 0; j < MT; ++j) r[q][j] = ns_frag<64, PL, false>(st, q, wc + j * 16, lane);
-        }
+        NsFrags<2, MT> f;
+        ns_read<64, 2, PL, false>(f.l, lane_l + s * STAGE);
+        ns_read<64, MT, PL, false>(f.r, lane_r + s * STAGE);
 #pragma unroll
         for (int j = 0; j < MT; ++j)
             if ((wc + j * 16) / SK == s) {                            // uniform
@@ -674,13 +717,7 @@ __device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* 
                     if constexpr (PL == 2) al[i][j] = *reinterpret_cast<const half4*>(st + place(rr, c, 1));
                 }
             }
-#pragma unroll
-        for (int q = 0; q < (PL == 2 ? 3 : 2); ++q)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < MT; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r[PL == 2 ? q == 1 : q][j], l[PL == 2 ? q == 2 : q][i], acc[i][j], 0, 0, 0);
+        ns_mfma<false>(f, acc);
     };
     // stage s has landed when at most what was issued behind it is outstanding
     auto first_half = [&](auto self, auto at) {
@@ -723,11 +760,12 @@ __device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* 
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
             const int r = wr + i * 16 + (lane & 15), c = wc + j * 16 + (lane >> 4) * 4;
+            const f32x4 sq = acc.get(i, j);
             half4 h, l;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 half_t x, y;
-                split_half(fmaf(f1, (float)ah[i][j][e] + (float)al[i][j][e], acc[i][j][e] * f0) + (band + r == c + e ? f2 : 0.f), x, y);
+                split_half(ns_poly(poly, sq[e], (float)ah[i][j][e] + (float)al[i][j][e], band + r == c + e), x, y);
                 h[e] = x;
                 l[e] = y;
             }
@@ -737,23 +775,18 @@ __device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* 
         }
     ns_wait<0, true>();                                               // X's tile has landed, the band is written
     ns_barrier();
-    f32x4 out[2][1];
-    out[0][0] = out[1][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+    NsSums<2, 1, PL, true> out;
+    out.clear();
     const int o_r = (wave >> 2) * 32, o_c = (wave & 3) * 16;
     auto last = [&](auto tall) {
         constexpr bool TALL = decltype(tall)::value;
+        const unsigned ol = ns_lane<64, PL, false>(smem + (TALL ? X_AT : P_AT), o_r, lane), o_right = ns_lane<64, PL, !TALL>(smem + (TALL ? P_AT : X_AT), o_c, lane);
 #pragma unroll
         for (int s = 0; s < KT; ++s) {
-            const unsigned char *P = smem + P_AT + s * X_STAGE, *Xs = smem + X_AT + s * X_STAGE;
             NsFrags<2, 1> f;
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) f.l[q][i] = ns_frag<64, PL, false>(TALL ? Xs : P, q, o_r + i * 16, lane);
-                if constexpr (TALL) f.r[q][0] = ns_frag<64, PL, false>(P, q, o_c, lane);
-                else f.r[q][0] = ns_frag<64, PL, true>(Xs, q, o_c, lane);
-            }
-            ns_mfma<2, 1, PL>(f, out);
+            ns_read<64, 2, PL, false>(f.l, ol + s * X_STAGE);
+            ns_read<64, 1, PL, !TALL>(f.r, o_right + s * X_STAGE);
+            ns_mfma<false>(f, out);
         }
     };
     if (d.tall) last(std::true_type());
@@ -762,14 +795,14 @@ __device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* 
     ns_barrier();                                                     // the operands have been read: the tile in fp32 goes to the front
     float* S = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) *reinterpret_cast<f32x4*>(S + (o_r + i * 16 + (lane & 15)) * SMALL_PITCH + o_c + (lane >> 4) * 4) = out[i][0];
+    for (int i = 0; i < 2; ++i) *reinterpret_cast<f32x4*>(S + (o_r + i * 16 + (lane & 15)) * SMALL_PITCH + o_c + (lane >> 4) * 4) = out.get(i, 0);
     __syncthreads();
 }
 template <int PL, int EPI>
 __global__ __launch_bounds__(512, 1) void ns_small_kernel(
-    const NsTable t, const NsPtrs p, half_t* __restrict__ ws, const float* __restrict__ hyper, int which, float f0, float f1, float f2, float g0, int low,
-    int zero_grad) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const NsTable t, const NsPtrs p, half_t* __restrict__ ws, const float* __restrict__ hyper, int which, const NsScale poly,
+    const NsScale f) {
+    extern __shared__ __attribute__((aligned(512))) unsigned char smem[];
     NsPlace w;
     if (!ns_place(t, w)) return;
     const int it = w.it, mat = w.mat, tile = w.tile;
@@ -778,9 +811,9 @@ __global__ __launch_bounds__(512, 1) void ns_small_kernel(
     const int tc = d.cp / 64, ti = tile / tc, tj = tile - ti * tc, tid = threadIdx.x;
     half_t* base = ws + d.ws + mat * d.wsz;
     const half_t *A = base + off_a(d), *X = base + off_x(d, which);
-    if (d.mp == 192) ns_small_product<3, PL>(A, X, d, ti, tj, f0, f1, f2, smem);
-    else if (d.mp == 128) ns_small_product<2, PL>(A, X, d, ti, tj, f0, f1, f2, smem);
-    else ns_small_product<1, PL>(A, X, d, ti, tj, f0, f1, f2, smem);
+    if (d.mp == 192) ns_small_product<3, PL>(A, X, d, ti, tj, poly, smem);
+    else if (d.mp == 128) ns_small_product<2, PL>(A, X, d, ti, tj, poly, smem);
+    else ns_small_product<1, PL>(A, X, d, ti, tj, poly, smem);
     float lr = 0.f, keep = 1.f;
     if constexpr (EPI == EPI_UPDATE) { lr = hyper[0]; keep = 1.f - lr * hyper[2]; lr *= p.scale[it]; }
     const int lrow = tid >> 3, lcol = (tid & 7) * 8, r = ti * 64 + lrow, c = tj * 64 + lcol;
@@ -789,12 +822,12 @@ __global__ __launch_bounds__(512, 1) void ns_small_kernel(
         const float* sp = reinterpret_cast<const float*>(smem) + lrow * SMALL_PITCH + lcol;
         const f32x4 a = *reinterpret_cast<const f32x4*>(sp), b = *reinterpret_cast<const f32x4*>(sp + 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { v[e] = a[e] * g0; v[4 + e] = b[e] * g0; }
+        for (int e = 0; e < 4; ++e) { v[e] = a[e] * f.f0; v[4 + e] = b[e] * f.f0; }
     }
-    if constexpr (EPI == EPI_MULT) ns_store8(base + off_x(d, which ^ 1), low, r, c, d.cp, v);
+    if constexpr (EPI == EPI_MULT) ns_store8(base + off_x(d, which ^ 1), f.low, r, c, d.cp, v);
     else {
         const int n = r < d.rows ? (d.cols - c < 8 ? d.cols - c : 8) : 0;
-        if (n > 0) ns_finish8<EPI>(p, it, mat, r, c, n, lr, keep, zero_grad, v);
+        if (n > 0) ns_finish8<EPI>(p, it, mat, r, c, n, lr, keep, f.zero_grad, v);
     }
 }
 
@@ -874,7 +907,6 @@ double ns_bounds(double bound, double a, double b, double c, double& pmax) {
     return xmax > 1e-3 ? xmax * 1.01 : 1e-3;
 }
 
-struct NsScale { float f0, f1, f2; int low, zero_grad; };
 // Which tile a launch takes: the shortest estimate from times measured on pairs of planes, in us: 5 for a tile's start and end, plus per 32 k
 // (n tiles on 256 CUs)                 64 x 64: 0.225, alone on its CU
 //   128 x 128: 0.85 alone, 1.15 for two on a CU             128 x 64: 0.5 alone, 0.75 for two, 1.1 for three.
@@ -911,7 +943,7 @@ int launch_gemm_v(NsTable& t, const NsPtrs& p, half_t* ws, const float* hyper, i
     S3D_REQUIRE(grid >= 0, "newton_schulz: too many tiles");
     auto k = ns_gemm_kernel<KIND, PL, EPI>;
     if (Tile::BYTES > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, Tile::BYTES);
-    hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(256), Tile::BYTES, s, t, p, ws, hyper, which, f.f0, f.f1, f.f2, f.low, f.zero_grad);
+    hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(256), Tile::BYTES, s, t, p, ws, hyper, which, f);
     S3D_CHECK_LAUNCH_V("newton_schulz", KIND * 100 + PL * 10 + EPI);
     return 0;
 }
@@ -943,7 +975,7 @@ int launch_small(NsPlan& pl, const NsPtrs& p, half_t* ws, const float* hyper, in
     S3D_REQUIRE(grid >= 0, "newton_schulz: too many tiles");
     auto k = ns_small_kernel<PL, EPI>;
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_BYTES);
-    hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(512), SMALL_BYTES, s, pl.t, p, ws, hyper, which, poly.f0, poly.f1, poly.f2, mult.f0, mult.low, mult.zero_grad);
+    hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(512), SMALL_BYTES, s, pl.t, p, ws, hyper, which, poly, mult);
     S3D_CHECK_LAUNCH_V("newton_schulz_small", PL * 10 + EPI);
     return 0;
 }
@@ -971,10 +1003,13 @@ int ns_run(NsPlan& pl, const NsPtrs& p, const S3dNsArgs& a, const float* hyper, 
     for (int k = 0; k < a.steps; ++k) {
         double pmax;
         const double next = ns_bounds(bound, a.a, a.b, a.c, pmax);
-        const float sa = pow2_under(32768., bound * bound), sp = pow2_under(32768., pmax), sn = pow2_under(32768., next);
+        // What is kept of A and squared is A - shift I, in the middle of the spectrum: P = c (A - shift)^2 + b' (A - shift) + a'.  Near the end, where the
+        // singular values are about 1, that square is a tenth of A^2 and so is what its sum loses (the whole result: a third less).
+        const double shift = 0.375 * bound * bound, a1 = a.a + (a.b + a.c * shift) * shift, b1 = a.b + 2. * a.c * shift;
+        const float sa = pow2_under(32768., bound * bound - shift), sp = pow2_under(32768., pmax), sn = pow2_under(32768., next);
         const int planes = k >= plain_from ? 1 : 2, low = planes == 2, low_x = k + 1 < plain_from;
-        if (int rc = launch_gemm<EPI_GRAM>(pl, planes, p, ws, hyper, k & 1, {sa / (sx * sx), 0.f, 0.f, low, 0}, s)) return rc;
-        const NsScale poly = {a.c * sp / (sa * sa), a.b * sp / sa, a.a * sp, low, 0}, mult = {sn / (sp * sx), 0.f, 0.f, low_x, 0}, last = {1.f / (sp * sx), 0.f, 0.f, 0, a.zero_grad};
+        if (int rc = launch_gemm<EPI_GRAM>(pl, planes, p, ws, hyper, k & 1, {sa / (sx * sx), 0.f, -(float)shift * sa, low, 0}, s)) return rc;
+        const NsScale poly = {a.c * sp / (sa * sa), (float)b1 * sp / sa, (float)a1 * sp, low, 0}, mult = {sn / (sp * sx), 0.f, 0.f, low_x, 0}, last = {1.f / (sp * sx), 0.f, 0.f, 0, a.zero_grad};
         const bool end = k + 1 == a.steps;
         int rc;
         if (small) {
