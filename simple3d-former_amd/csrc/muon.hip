@@ -439,12 +439,13 @@ __device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& 
     }
 }
 
-// The same for a 64 x 64 tile with the k range dealt to the four waves (stage s to wave s % 4): every wave works the whole tile on its own
+// The same for a 64 x 64 or 32 x 32 tile with the k range dealt to the four waves (stage s to wave s % 4): every wave works the whole tile on its own
 // stages, brought by itself, so nothing is waited for but its own loads; a quarter of the serial length and half the LDS reads per product.  The
-// four partial sums are added through LDS in the order of the waves.  out[j][e] = C[16 wave + (lane & 15)][16 j + 4 (lane >> 4) + e].
-template <int RING, int PL, bool LK, bool RK>
-__device__ __forceinline__ void ns_product_ksplit(const NsOperand& L, const NsOperand& R, int K, unsigned char* smem, f32x4 (&out)[4]) {
-    constexpr int T = 64, STAGE = 2 * T * 128, PIECES = STAGE / 1024, F = 4;
+// four partial sums are added through LDS in the order of the waves.  64: out[j][e] = C[16 wave + (lane & 15)][16 j + 4 (lane >> 4) + e]; 32: out[0][e] =
+// C[16 (wave >> 1) + (lane & 15)][16 (wave & 1) + 4 (lane >> 4) + e].
+template <int T, int RING, int PL, bool LK, bool RK>
+__device__ __forceinline__ void ns_product_ksplit(const NsOperand& L, const NsOperand& R, int K, unsigned char* smem, f32x4 (&out)[T * T / 1024]) {
+    constexpr int STAGE = 2 * T * 128, PIECES = STAGE / 1024, F = T / 16, MINE = F * F / 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     unsigned char* mine = smem + wave * RING * STAGE;
     const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)mine);
@@ -476,7 +477,7 @@ __device__ __forceinline__ void ns_product_ksplit(const NsOperand& L, const NsOp
         slot = slot == (RING - 1) * STAGE ? 0 : slot + STAGE;
         ns_mfma<false>(f, acc);
     }
-    // partial sums: 16 KB per wave in its own ring (read by nobody any more), then rows 16 wave .. + 15 from all four
+    // partial sums: T x T per wave in its own ring (read by nobody any more), then a quarter of the tile from all four
     f32x4* red = reinterpret_cast<f32x4*>(mine);
 #pragma unroll
     for (int i = 0; i < F; ++i)
@@ -484,25 +485,28 @@ __device__ __forceinline__ void ns_product_ksplit(const NsOperand& L, const NsOp
         for (int j = 0; j < F; ++j) red[(i * F + j) * 64 + lane] = acc.get(i, j);
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < F; ++j) {
+    for (int j = 0; j < MINE; ++j) {
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) v += reinterpret_cast<const f32x4*>(smem + w * RING * STAGE)[(wave * F + j) * 64 + lane];
+        for (int w = 0; w < 4; ++w) v += reinterpret_cast<const f32x4*>(smem + w * RING * STAGE)[(wave * MINE + j) * 64 + lane];
         out[j] = v;
     }
 }
 
 // How a tile is worked.  TILE_128: 128 x 128, four waves, 66 KB of LDS: two workgroups share a CU, one's start and epilogue lie under the other's
 // products.  TILE_HALF: 128 x 64, 48 KB, three on a CU: half the granularity for half again the LDS traffic per product.  TILE_64: 64 x 64, the
-// k range over the four waves: launches with too few tiles for the CUs.
-enum { TILE_128 = 0, TILE_64 = 1, TILE_HALF = 2 };
+// k range over the four waves: launches with too few tiles for the CUs.  TILE_32 the same with 32 x 32 (Gram products of pairs): launches with so few that
+// what one CU can fetch is the bound.
+enum { TILE_128 = 0, TILE_64 = 1, TILE_HALF = 2, TILE_32 = 3 };
 template <int KIND>
 struct NsTile {
-    static constexpr int TR = KIND == TILE_64 ? 64 : 128, TC = KIND == TILE_128 ? 128 : 64, PITCH = TC + 4;
+    static constexpr bool KSPLIT = KIND == TILE_64 || KIND == TILE_32;
+    static constexpr int TR = KIND == TILE_64 ? 64 : KIND == TILE_32 ? 32 : 128, TC = KIND == TILE_HALF ? 64 : TR, PITCH = TC + 4;
+    static constexpr int RING = KIND == TILE_32 ? 4 : 2;
     static constexpr int SUM_BYTES = TR * PITCH * 4;                 // the tile in fp32
-    static constexpr int RING_BYTES = KIND == TILE_64 ? 4 * 2 * 16384 : 2 * (TR + TC) * 128;
-    static constexpr int SUM_AT = KIND == TILE_64 ? RING_BYTES : 0;  // over the ring, except where the ring still holds partial sums
-    static constexpr int BYTES = KIND == TILE_64 ? RING_BYTES + SUM_BYTES : SUM_BYTES > RING_BYTES ? SUM_BYTES : RING_BYTES;
+    static constexpr int RING_BYTES = (KSPLIT ? 4 : 1) * RING * (TR + TC) * 128;
+    static constexpr int SUM_AT = KSPLIT ? RING_BYTES : 0;           // over the ring, except where the ring still holds partial sums
+    static constexpr int BYTES = KSPLIT ? RING_BYTES + SUM_BYTES : SUM_BYTES > RING_BYTES ? SUM_BYTES : RING_BYTES;
 };
 
 // 8 elements of a tensor of the iteration at column c (a multiple of 8), stored as a pair or as one plane
@@ -546,7 +550,7 @@ struct NsScale { float f0, f1, f2; int low, zero_grad; };
 __device__ __forceinline__ float ns_poly(const NsScale& f, float square, float a, bool diagonal) { return fmaf(f.f1, a, f.f0 * square) + (diagonal ? f.f2 : 0.f); }
 
 template <int KIND, int PL, int EPI>
-__global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_128 ? 2 : 3) void ns_gemm_kernel(
+__global__ __launch_bounds__(256, NsTile<KIND>::KSPLIT ? 1 : KIND == TILE_128 ? 2 : 3) void ns_gemm_kernel(
     const NsTable t, const NsPtrs p, half_t* __restrict__ ws, const float* __restrict__ hyper, int which, const NsScale f) {
     extern __shared__ __attribute__((aligned(512))) unsigned char smem[];
     using Tile = NsTile<KIND>;
@@ -575,14 +579,18 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_128 ? 2 : 3
     float* S = reinterpret_cast<float*>(smem + Tile::SUM_AT);        // the tile, [TR][PITCH]
     auto product = [&](auto lk, auto rk, const NsOperand& L, const NsOperand& R, int K) {
         constexpr bool LK = decltype(lk)::value, RK = decltype(rk)::value;
-        if constexpr (KIND == TILE_64) {
+        if constexpr (KIND == TILE_32) {
+            f32x4 acc[1];
+            ns_product_ksplit<TR, Tile::RING, PL, LK, RK>(L, R, K, smem, acc);
+            *reinterpret_cast<f32x4*>(S + ((wave >> 1) * 16 + (lane & 15)) * PITCH + (wave & 1) * 16 + (lane >> 4) * 4) = acc[0];
+        } else if constexpr (KIND == TILE_64) {
             f32x4 acc[4];
-            ns_product_ksplit<2, PL, LK, RK>(L, R, K, smem, acc);
+            ns_product_ksplit<TR, Tile::RING, PL, LK, RK>(L, R, K, smem, acc);
 #pragma unroll
             for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(S + (wave * 16 + (lane & 15)) * PITCH + j * 16 + (lane >> 4) * 4) = acc[j];
         } else {
             NsSums<TR / 32, TC / 32, PL, false> acc;
-            ns_product<TR, TC, 2, PL, LK, RK>(L, R, K, smem, acc);
+            ns_product<TR, TC, Tile::RING, PL, LK, RK>(L, R, K, smem, acc);
             float* mine = S + ((wave >> 1) * (TR / 2) + (lane & 15)) * PITCH + (wave & 1) * (TC / 2) + (lane >> 4) * 4;
             __syncthreads();                                         // every wave has read its last stage: the ring is free
 #pragma unroll
@@ -907,15 +915,17 @@ double ns_bounds(double bound, double a, double b, double c, double& pmax) {
     return xmax > 1e-3 ? xmax * 1.01 : 1e-3;
 }
 
-// Which tile a launch takes: the shortest estimate from times measured on pairs of planes, in us: 5 for a tile's start and end, plus per 32 k
+// Which tile a launch takes.  32 x 32 for Gram products of pairs whose tiles fit on the CUs once over: a 64 x 64 tile of k = 768 fetches 393 KB through
+// one CU (64 / 32, us for one launch: 192 x 192, 6 / 21 tiles, 7.0 / 4.9; the four matrices of a 192-wide block, 24 / 84 tiles, 10.9 / 6.6).  Else the shortest estimate from times measured on pairs of planes, in us: 5 for a tile's start and end, plus per 32 k
 // (n tiles on 256 CUs)                 64 x 64: 0.225, alone on its CU
 //   128 x 128: 0.85 alone, 1.15 for two on a CU             128 x 64: 0.5 alone, 0.75 for two, 1.1 for three.
 // Measured, 64 / 128 for the whole chain of five steps (tiles of 128 in the symmetric products / in P X): 12 x 384^2 (72 / 108) 166 / 236, 16 x 384^2
 // (96 / 144) 251 / 239, 4 x 768^2 (84 / 144) 326 / 354, 12 x 768^2 (252 / 432) 657 / 469, 8 x 384 x 1536 (48 / 288) 277 / 374, 16 x (96 / 576) 493 / 439.
 // 128 x 128 / 128 x 64 for one launch: the four products of twelve 384-wide blocks, Gram 52 / 48, polynomial 27 / 25, P X 63 / 67; 4 x 2048^2, Gram
 // 126 / 121, polynomial 130 / 123, P X 179 / 197; ragged stacks of 192 tiles, P X 15 / 12.
-int tile_kind(const NsTable& t, bool gram, bool sym, int planes) {
+int tile_kind(const NsTable& t, bool large, bool gram, bool sym, int planes) {
     struct Sum { double n = 0., alone = 0., two = 0., three = 0.; } s64, s128, half;
+    double n32 = 0.;
     auto add = [](Sum& s, double n, double stages, double alone, double two, double three) {
         s.n += n;
         s.two += n * (5. + two * stages);
@@ -925,14 +935,18 @@ int tile_kind(const NsTable& t, bool gram, bool sym, int planes) {
     for (int i = 0; i < t.n; ++i) {
         const NsDims& d = t.d[i];
         const double stages = (gram ? (d.tall ? d.rp : d.cp) : d.mp) * (planes == 2 ? 1. : 0.5) / 32;
-        const double m6 = d.mp / 64, m12 = d.mp / 128;
+        const double m3 = d.mp / 32, m6 = d.mp / 64, m12 = d.mp / 128;
         const double a = d.count * (sym ? m6 * (m6 + 1) / 2 : (double)(d.rp / 64) * (d.cp / 64));
         const double b = d.count * (sym ? m12 * (m12 + 1) / 2 : (double)(d.rp / 128) * (d.cp / 128));
+        n32 += d.count * m3 * (m3 + 1) / 2;
         add(s64, a, stages, 0.225, 0.225, 0.);
         add(s128, b, stages, 0.85, 1.15, 0.);
         add(half, 2. * b, stages, 0.5, 0.75, 1.1);
     }
-    const double t64 = ceil(s64.n / 256) * s64.two / s64.n, t128 = s128.n <= 256 ? s128.alone : ceil(s128.n / 512) * s128.two / s128.n;
+    if (gram && planes == 2 && n32 <= 256) return TILE_32;
+    const double t64 = ceil(s64.n / 256) * s64.two / s64.n;
+    if (!large) return TILE_64;
+    const double t128 = s128.n <= 256 ? s128.alone : ceil(s128.n / 512) * s128.two / s128.n;
     const double th = half.n <= 256 ? half.alone : half.n <= 512 ? fmax(half.alone, half.two / half.n) : ceil(half.n / 768) * half.three / half.n;
     return th < t64 && th < t128 ? TILE_HALF : t128 < t64 ? TILE_128 : TILE_64;
 }
@@ -949,7 +963,9 @@ int launch_gemm_v(NsTable& t, const NsPtrs& p, half_t* ws, const float* hyper, i
 }
 template <int EPI>
 int launch_gemm(NsPlan& pl, int planes, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& f, hipStream_t s) {
-    const int kind = pl.pad == 128 ? tile_kind(pl.t, EPI == EPI_GRAM, EPI == EPI_GRAM || EPI == EPI_POLY, planes) : TILE_64;
+    const int kind = tile_kind(pl.t, pl.pad == 128, EPI == EPI_GRAM, EPI == EPI_GRAM || EPI == EPI_POLY, planes);
+    if constexpr (EPI == EPI_GRAM)
+        if (kind == TILE_32) return launch_gemm_v<TILE_32, 2, EPI>(pl.t, p, ws, hyper, which, f, s);
 #define S3D_NS_CASE(k)                                                                                 \
     if (kind == k) return planes == 2 ? launch_gemm_v<k, 2, EPI>(pl.t, p, ws, hyper, which, f, s)      \
                                       : launch_gemm_v<k, 1, EPI>(pl.t, p, ws, hyper, which, f, s);
