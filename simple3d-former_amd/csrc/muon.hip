@@ -916,7 +916,8 @@ double ns_bounds(double bound, double a, double b, double c, double& pmax) {
 }
 
 // Which tile a launch takes.  32 x 32 for Gram products of pairs whose tiles fit on the CUs once over: a 64 x 64 tile of k = 768 fetches 393 KB through
-// one CU (64 / 32, us for one launch: 192 x 192, 6 / 21 tiles, 7.0 / 4.9; the four matrices of a 192-wide block, 24 / 84 tiles, 10.9 / 6.6).  Else the shortest estimate from times measured on pairs of planes, in us: 5 for a tile's start and end, plus per 32 k
+// one CU (64 / 32, us for one launch: 192 x 192, 6 / 21 tiles, 7.0 / 4.9; the four matrices of a 192-wide block, 24 / 84 tiles, 10.9 / 6.6).
+// Else the shortest estimate from times measured on pairs of planes, in us: 5 for a tile's start and end, plus per 32 k
 // (n tiles on 256 CUs)                 64 x 64: 0.225, alone on its CU
 //   128 x 128: 0.85 alone, 1.15 for two on a CU             128 x 64: 0.5 alone, 0.75 for two, 1.1 for three.
 // Measured, 64 / 128 for the whole chain of five steps (tiles of 128 in the symmetric products / in P X): 12 x 384^2 (72 / 108) 166 / 236, 16 x 384^2
@@ -938,12 +939,12 @@ int tile_kind(const NsTable& t, bool large, bool gram, bool sym, int planes) {
         const double m3 = d.mp / 32, m6 = d.mp / 64, m12 = d.mp / 128;
         const double a = d.count * (sym ? m6 * (m6 + 1) / 2 : (double)(d.rp / 64) * (d.cp / 64));
         const double b = d.count * (sym ? m12 * (m12 + 1) / 2 : (double)(d.rp / 128) * (d.cp / 128));
-        n32 += d.count * m3 * (m3 + 1) / 2;
+        n32 += d.count * (sym ? m3 * (m3 + 1) / 2 : (double)(d.rp / 32) * (d.cp / 32));
         add(s64, a, stages, 0.225, 0.225, 0.);
         add(s128, b, stages, 0.85, 1.15, 0.);
         add(half, 2. * b, stages, 0.5, 0.75, 1.1);
     }
-    if (gram && planes == 2 && n32 <= 256) return TILE_32;
+    if (planes == 2 && n32 <= 256) return TILE_32;
     const double t64 = ceil(s64.n / 256) * s64.two / s64.n;
     if (!large) return TILE_64;
     const double t128 = s128.n <= 256 ? s128.alone : ceil(s128.n / 512) * s128.two / s128.n;
@@ -964,8 +965,7 @@ int launch_gemm_v(NsTable& t, const NsPtrs& p, half_t* ws, const float* hyper, i
 template <int EPI>
 int launch_gemm(NsPlan& pl, int planes, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& f, hipStream_t s) {
     const int kind = tile_kind(pl.t, pl.pad == 128, EPI == EPI_GRAM, EPI == EPI_GRAM || EPI == EPI_POLY, planes);
-    if constexpr (EPI == EPI_GRAM)
-        if (kind == TILE_32) return launch_gemm_v<TILE_32, 2, EPI>(pl.t, p, ws, hyper, which, f, s);
+    if (kind == TILE_32) return launch_gemm_v<TILE_32, 2, EPI>(pl.t, p, ws, hyper, which, f, s);
 #define S3D_NS_CASE(k)                                                                                 \
     if (kind == k) return planes == 2 ? launch_gemm_v<k, 2, EPI>(pl.t, p, ws, hyper, which, f, s)      \
                                       : launch_gemm_v<k, 1, EPI>(pl.t, p, ws, hyper, which, f, s);
