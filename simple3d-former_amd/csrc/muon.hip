@@ -502,7 +502,7 @@ template <int KIND>
 struct NsTile {
     static constexpr bool KSPLIT = KIND == TILE_64 || KIND == TILE_32;
     static constexpr int TR = KIND == TILE_64 ? 64 : KIND == TILE_32 ? 32 : 128, TC = KIND == TILE_HALF ? 64 : TR, PITCH = TC + 4;
-    static constexpr int RING = KIND == TILE_32 ? 4 : 2;
+    static constexpr int RING = 2;
     static constexpr int SUM_BYTES = TR * PITCH * 4;                 // the tile in fp32
     static constexpr int RING_BYTES = (KSPLIT ? 4 : 1) * RING * (TR + TC) * 128;
     static constexpr int SUM_AT = KSPLIT ? RING_BYTES : 0;           // over the ring, except where the ring still holds partial sums
@@ -550,7 +550,7 @@ struct NsScale { float f0, f1, f2; int low, zero_grad; };
 __device__ __forceinline__ float ns_poly(const NsScale& f, float square, float a, bool diagonal) { return fmaf(f.f1, a, f.f0 * square) + (diagonal ? f.f2 : 0.f); }
 
 template <int KIND, int PL, int EPI>
-__global__ __launch_bounds__(256, NsTile<KIND>::KSPLIT ? 1 : KIND == TILE_128 ? 2 : 3) void ns_gemm_kernel(
+__global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_HALF ? 3 : 2) void ns_gemm_kernel(
     const NsTable t, const NsPtrs p, half_t* __restrict__ ws, const float* __restrict__ hyper, int which, const NsScale f) {
     extern __shared__ __attribute__((aligned(512))) unsigned char smem[];
     using Tile = NsTile<KIND>;
@@ -915,8 +915,9 @@ double ns_bounds(double bound, double a, double b, double c, double& pmax) {
     return xmax > 1e-3 ? xmax * 1.01 : 1e-3;
 }
 
-// Which tile a launch takes.  32 x 32 for Gram products of pairs whose tiles fit on the CUs once over: a 64 x 64 tile of k = 768 fetches 393 KB through
-// one CU (64 / 32, us for one launch: 192 x 192, 6 / 21 tiles, 7.0 / 4.9; the four matrices of a 192-wide block, 24 / 84 tiles, 10.9 / 6.6).
+// Which tile a launch takes.  32 x 32, two on a CU, for products of pairs whose tiles fit on the CUs once over: a 64 x 64 tile of k = 768 fetches 393 KB
+// through one CU (64 / 32, us for one Gram launch: 192 x 192, 6 / 21 tiles, 7.0 / 4.9; the four matrices of a 192-wide block, 24 / 84, 10.9 / 6.6.  Whole
+// chains: 2 x 384^2 116 / 90, 512^2 128 / 92, 768^2 169 / 142, 700 x 3000 280 / 250).
 // Else the shortest estimate from times measured on pairs of planes, in us: 5 for a tile's start and end, plus per 32 k
 // (n tiles on 256 CUs)                 64 x 64: 0.225, alone on its CU
 //   128 x 128: 0.85 alone, 1.15 for two on a CU             128 x 64: 0.5 alone, 0.75 for two, 1.1 for three.
@@ -944,7 +945,7 @@ int tile_kind(const NsTable& t, bool large, bool gram, bool sym, int planes) {
         add(s128, b, stages, 0.85, 1.15, 0.);
         add(half, 2. * b, stages, 0.5, 0.75, 1.1);
     }
-    if (planes == 2 && n32 <= 256) return TILE_32;
+    if (planes == 2 && n32 <= 512) return TILE_32;
     const double t64 = ceil(s64.n / 256) * s64.two / s64.n;
     if (!large) return TILE_64;
     const double t128 = s128.n <= 256 ? s128.alone : ceil(s128.n / 512) * s128.two / s128.n;
