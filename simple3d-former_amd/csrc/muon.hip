@@ -917,7 +917,8 @@ double ns_bounds(double bound, double a, double b, double c, double& pmax) {
 
 // Which tile a launch takes.  32 x 32, two on a CU, for products of pairs whose tiles fit on the CUs once over: a 64 x 64 tile of k = 768 fetches 393 KB
 // through one CU (64 / 32, us for one Gram launch: 192 x 192, 6 / 21 tiles, 7.0 / 4.9; the four matrices of a 192-wide block, 24 / 84, 10.9 / 6.6.  Whole
-// chains: 2 x 384^2 116 / 90, 512^2 128 / 92, 768^2 169 / 142, 700 x 3000 280 / 250).
+// chains: 2 x 384^2 116 / 90, 512^2 128 / 92, 768^2 169 / 142, 700 x 3000 280 / 250), or nearly so if k is short (513 .. 560 tiles: k = 576 163 / 153, ragged
+// stacks 178 / 170; k = 1024 190 / 204, k = 4000 371 / 445).
 // Else the shortest estimate from times measured on pairs of planes, in us: 5 for a tile's start and end, plus per 32 k
 // (n tiles on 256 CUs)                 64 x 64: 0.225, alone on its CU
 //   128 x 128: 0.85 alone, 1.15 for two on a CU             128 x 64: 0.5 alone, 0.75 for two, 1.1 for three.
@@ -945,7 +946,7 @@ int tile_kind(const NsTable& t, bool large, bool gram, bool sym, int planes) {
         add(s128, b, stages, 0.85, 1.15, 0.);
         add(half, 2. * b, stages, 0.5, 0.75, 1.1);
     }
-    if (planes == 2 && n32 <= 512) return TILE_32;
+    if (planes == 2 && (n32 <= 512 || (n32 <= 640 && s64.two <= 12. * s64.n))) return TILE_32;
     const double t64 = ceil(s64.n / 256) * s64.two / s64.n;
     if (!large) return TILE_64;
     const double t128 = s128.n <= 256 ? s128.alone : ceil(s128.n / 512) * s128.two / s128.n;
