@@ -11,9 +11,13 @@
 // Precision.  A step multiplies a small singular value by a = 3.4 and with it every rounding that fell into its direction: five steps
 // turn one rounding of the operands to bf16 into 3.4^5 * 2^-9 = 90 % of a direction, to fp16 into 10 %.  Operands are therefore PAIRS of fp16 planes
 // (hi = rne(x s), lo = rne(x s - hi), 22 bits; s a power of two that keeps the largest possible entry below 2^15) multiplied as
-// hi hi + hi lo + lo hi with fp32 accumulation: an fp32 product at a third of the fp16 matrix rate, five times that of the fp32 matrix
+// hi lo + lo hi + hi hi with fp32 accumulation: an fp32 product at a third of the fp16 matrix rate, five times that of the fp32 matrix
 // instructions.  fp16 planes rather than bf16: all entries are bounded by the spectral norm, so the exponent range is not needed and
 // the six extra bits are.
+//
+// Bound: the matrix cores for large stacks (4 x 2048^2: P X 161 - 200 us = 1030 - 1280 TF of fp16 products, a large library product 1095), the balance of uneven
+// k over the CUs for a model's (48 matrices, 384 wide: Gram 48 us of 30, P X 63 of 45, the last product HBM: 425 MB in 87 us), what one CU can fetch and
+// the latency of dependent launches for few small ones (192 x 192: twelve launches of 4 - 9 us, 74 us).
 #include <math.h>
 #include <stdlib.h>
 #include <string.h>

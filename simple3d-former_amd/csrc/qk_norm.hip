@@ -5,7 +5,8 @@
 // or (2i, 2i + 1) -- by the token's angles.  Backward: dz = R^T dy, dg += dz x r, d = dz g, dx = r (d - x r mean(d x r)).
 // Nothing but x is kept for the backward: r is one reduction over values it reads anyway.
 //
-// Bound: HBM.  One pass, every element read and written once in 16-byte pieces; the angles come from a table of [positions][hd/2] cosines and
+// Bound: HBM (188160 tokens of 9 heads of 256: forward 1.73 GB in 357 us = 4.85 TB/s, backward 2.6 GB in 480 us = 5.4 TB/s with the gains' reduction, a
+// large copy runs at 4.73), launch and host for few tokens (26: 4 us of kernel).  One pass, every element read and written once in 16-byte pieces; the angles come from a table of [positions][hd/2] cosines and
 // sines that stays in the caches.  A head is worked by G = 1 .. 16 lanes (hd / 16 rounded up to a power of two): each holds 8 elements of
 // either half, i.e. 8 whole pairs, so the rotation needs no exchange and the mean is log2(G) lane exchanges.  A workgroup works the query, the
 // key or the value heads of a range of rows (blockIdx.y): one gain and one gain gradient in registers, no divergence, and three times the
