@@ -59,7 +59,7 @@ struct NsPtrs {
     float scale[NS_ITEMS];
 };
 enum { SRC_F32 = 0, SRC_BF16 = 1, SRC_MUON = 2 };
-enum { EPI_GRAM = 0, EPI_POLY = 1, EPI_MULT = 2, EPI_OUT_F32 = 3, EPI_OUT_BF16 = 4, EPI_UPDATE = 5 };
+enum { EPI_GRAM = 0, EPI_POLY = 1, EPI_MULT = 2, EPI_OUT_F32 = 3, EPI_OUT_BF16 = 4, EPI_UPDATE = 5, EPI_GRAM_ROWS = 6 };      // _ROWS: no stack is tall
 
 // Workgroups go round robin over the eight XCDs, each with an L2 of its own: XCD x takes the x-th eighth of every stack's workgroups, so that the
 // tiles of one matrix share an L2 and the XCDs have equal shares of long and short products.  The grid is 8 * sum of ceil(wgs / 8): false for
@@ -257,17 +257,30 @@ __global__ __launch_bounds__(256) void ns_load_kernel(const NsTable t, const NsP
 struct NsOperand { const half_t* p; int ld, at; };
 
 // One stage of an operand is T x 128 bytes of LDS: T rows of one line (k-contiguous), or 32 (pairs) / 64 k rows of the tile's columns (k-major).
-// Piece q of it is 1 KB = one DMA instruction of a wave; every lane brings 16 bytes, the slot swizzle is applied here.
+// Piece q of it is 1 KB = one DMA instruction of a wave; every lane brings 16 bytes, the slot swizzle is applied here.  A lane's byte offset from ns_base is
+// (ns_lane_source ^ ns_flip(q)) + q * rows of a piece * row: the swizzles are linear in the row's bits and a row is a multiple of what they permute, so a
+// wave keeps one register for all its pieces.
 template <int T, int PL, bool KM>
-__device__ __forceinline__ unsigned ns_source(const NsOperand& o, int piece, int lane) {           // byte offset from ns_base (at most 128 rows)
-    if constexpr (KM) {
-        constexpr int W = PL * T, WK = W / 8;                        // halves / 16-byte slots of a row
-        const int r = piece * (64 / WK) + lane / WK, chunk = (lane % WK) ^ kmajor_swz<W>(r);
-        return (unsigned)(r * PL * o.ld + chunk * 8) * 2;
-    } else {
-        const int r = piece * 8 + (lane >> 3), chunk = (lane & 7) ^ dma_swz64(r);
-        return (unsigned)(r * PL * o.ld + chunk * 8) * 2;
-    }
+struct NsPieces {
+    static constexpr int W = PL * T, WK = W / 8;                     // k-major: halves / 16-byte slots of a row
+    static constexpr int ROWS = KM ? 64 / WK : 8;                    // of a piece
+};
+template <int T, int PL, bool KM>
+__device__ __forceinline__ unsigned ns_lane_source(const NsOperand& o, int lane) {
+    using P = NsPieces<T, PL, KM>;
+    const int r = KM ? lane / P::WK : lane >> 3, chunk = KM ? (lane % P::WK) ^ kmajor_swz<P::W>(r) : (lane & 7) ^ dma_swz64(r);
+    return (unsigned)(r * PL * o.ld + chunk * 8) * 2;
+}
+template <int T, int PL, bool KM>
+__device__ __forceinline__ unsigned ns_flip(int piece) {
+    using P = NsPieces<T, PL, KM>;
+    return (KM ? kmajor_swz<P::W>(piece * P::ROWS) : dma_swz64(piece * P::ROWS)) * 16;
+}
+template <int T, int PL, bool KM>
+__device__ __forceinline__ int ns_advance(const NsOperand& o, int piece) { return piece * NsPieces<T, PL, KM>::ROWS * PL * o.ld; }      // in halves
+template <int T, int PL, bool KM>
+__device__ __forceinline__ unsigned ns_source(const NsOperand& o, int piece, int lane) {           // (at most 192 rows)
+    return (ns_lane_source<T, PL, KM>(o, lane) ^ ns_flip<T, PL, KM>(piece)) + (unsigned)ns_advance<T, PL, KM>(o, piece) * 2;
 }
 template <int PL, bool KM>
 __device__ __forceinline__ const half_t* ns_base(const NsOperand& o) { return o.p + (KM ? (long)o.at * PL : (long)o.at * PL * o.ld); }
@@ -386,20 +399,23 @@ __device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& 
     const int left = LEFT - wave * PIECES;                           // this wave's pieces below `left` are L's
     const long step_l = ns_step<PL, LK>(L), step_r = ns_step<PL, RK>(R);
     const half_t *src_l = ns_base<PL, LK>(L), *src_r = ns_base<PL, RK>(R);
-    unsigned off[PIECES];
+    const unsigned off_l = ns_lane_source<TR, PL, LK>(L, lane), off_r = ns_lane_source<TC, PL, RK>(R, lane);
+    auto bring = [&](unsigned at) {                                  // this wave's pieces of the next stage
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-        const int q = wave * PIECES + i;
-        off[i] = i < left ? ns_source<TR, PL, LK>(L, q, lane) : ns_source<TC, PL, RK>(R, q - LEFT, lane);
-    }
+        for (int i = 0; i < PIECES; ++i) {
+            const int ql = wave * PIECES + i, qr = ql - LEFT;
+            const half_t* src = i < left ? src_l + ns_advance<TR, PL, LK>(L, ql) : src_r + ns_advance<TC, PL, RK>(R, qr);
+            const unsigned off = i < left ? off_l ^ ns_flip<TR, PL, LK>(ql) : off_r ^ ns_flip<TC, PL, RK>(qr);
+            ns_dma(src, off, at + i * 1024);
+        }
+    };
     const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)smem + wave * PIECES * 1024);
     const int KT = K / (PL == 2 ? 32 : 64);
     unsigned slot_in = 0, slot = 0;                                  // in bytes
     auto advance = [](unsigned& s) { s = s == (RING - 1) * STAGE ? 0 : s + STAGE; };
     acc.clear();
     for (int k = 0; k < RING && k < KT; ++k) {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) ns_dma(i < left ? src_l : src_r, off[i], lds0 + slot_in + i * 1024);
+        bring(lds0 + slot_in);
         src_l += step_l;
         src_r += step_r;
         advance(slot_in);
@@ -424,9 +440,7 @@ __device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& 
         advance(slot);
         // the reads lie under the products (finer interleavings of loads, reads and products measured the same or slower)
         constexpr int M = ns_products<PL, FR, FC>();
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i)
-            if (more) ns_dma(i < left ? src_l : src_r, off[i], lds0 + slot_in + i * 1024);
+        if (more) bring(lds0 + slot_in);
         ns_mfma<FIRST>(now, acc, 0, M / 3);
         ns_read<TR, FR, PL, LK>(next.l, lane_l + slot);
         ns_mfma<FIRST>(now, acc, M / 3, 2 * M / 3);
@@ -499,7 +513,7 @@ __device__ __forceinline__ void ns_product_ksplit(const NsOperand& L, const NsOp
 
 // How a tile is worked.  TILE_128: 128 x 128, four waves, 66 KB of LDS: two workgroups share a CU, one's start and epilogue lie under the other's
 // products.  TILE_HALF: 128 x 64, 48 KB, three on a CU: half the granularity for half again the LDS traffic per product.  TILE_64: 64 x 64, the
-// k range over the four waves: launches with too few tiles for the CUs.  TILE_32 the same with 32 x 32 (Gram products of pairs): launches with so few that
+// k range over the four waves: launches with too few tiles for the CUs.  TILE_32 the same with 32 x 32 (pairs), 70 KB, two on a CU: launches with so few that
 // what one CU can fetch is the bound.
 enum { TILE_128 = 0, TILE_64 = 1, TILE_HALF = 2, TILE_32 = 3 };
 template <int KIND>
@@ -554,12 +568,12 @@ struct NsScale { float f0, f1, f2; int low, zero_grad; };
 __device__ __forceinline__ float ns_poly(const NsScale& f, float square, float a, bool diagonal) { return fmaf(f.f1, a, f.f0 * square) + (diagonal ? f.f2 : 0.f); }
 
 template <int KIND, int PL, int EPI>
-__global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_HALF ? 3 : 2) void ns_gemm_kernel(
+__global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_HALF && !(EPI == EPI_GRAM && PL == 2) ? 3 : 2) void ns_gemm_kernel(
     const NsTable t, const NsPtrs p, half_t* __restrict__ ws, const float* __restrict__ hyper, int which, const NsScale f) {
     extern __shared__ __attribute__((aligned(512))) unsigned char smem[];
     using Tile = NsTile<KIND>;
     constexpr int TR = Tile::TR, TC = Tile::TC, PITCH = Tile::PITCH, Q = TR / TC;
-    constexpr bool SYM = EPI == EPI_GRAM || EPI == EPI_POLY;
+    constexpr bool GRAM = EPI == EPI_GRAM || EPI == EPI_GRAM_ROWS, SYM = GRAM || EPI == EPI_POLY;
     NsPlace w;
     if (!ns_place(t, w)) return;
     const int it = w.it, mat = w.mat, tile = w.tile;
@@ -606,7 +620,8 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_HALF ? 3 : 
     };
     const std::false_type rows;                                      // operand stored as rows of k
     const std::true_type kmajor;
-    if constexpr (EPI == EPI_GRAM) {
+    if constexpr (EPI == EPI_GRAM_ROWS) product(rows, rows, NsOperand{X, d.cp, ti * TR}, NsOperand{X, d.cp, tj * TC}, d.cp);
+    else if constexpr (EPI == EPI_GRAM) {
         const NsOperand L = {X, d.cp, ti * TR}, R = {X, d.cp, tj * TC};
         if (!d.tall) product(rows, rows, L, R, d.cp);
         else product(kmajor, kmajor, L, R, d.rp);
@@ -620,7 +635,7 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_HALF ? 3 : 
     }
     float lr = 0.f, keep = 1.f;
     if constexpr (EPI == EPI_UPDATE) { lr = hyper[0]; keep = 1.f - lr * hyper[2]; lr *= p.scale[it]; }
-    half_t* O = base + (EPI == EPI_GRAM ? off_a(d) : EPI == EPI_POLY ? off_p(d) : off_x(d, which ^ 1));
+    half_t* O = base + (GRAM ? off_a(d) : EPI == EPI_POLY ? off_p(d) : off_x(d, which ^ 1));
     const int ld = SYM ? d.mp : d.cp;
     // rows of the tile, 8 columns per thread
 #pragma unroll 4
@@ -645,7 +660,7 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_HALF ? 3 : 
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] *= f.f0;
         }
-        if constexpr (EPI == EPI_GRAM) {
+        if constexpr (GRAM) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += r == c + e ? f.f2 : 0.f;
         }
@@ -923,14 +938,15 @@ double ns_bounds(double bound, double a, double b, double c, double& pmax) {
 // through one CU (64 / 32, us for one Gram launch: 192 x 192, 6 / 21 tiles, 7.0 / 4.9; the four matrices of a 192-wide block, 24 / 84, 10.9 / 6.6.  Whole
 // chains: 2 x 384^2 116 / 90, 512^2 128 / 92, 768^2 169 / 142, 700 x 3000 280 / 250), or nearly so if k is short (513 .. 560 tiles: k = 576 163 / 153, ragged
 // stacks 178 / 170; k = 1024 190 / 204, k = 4000 371 / 445).
-// Else the shortest estimate from times measured on pairs of planes, in us: 5 for a tile's start and end, plus per 32 k
+// Else the shortest estimate (Gram products of pairs with tall stacks among them, two k-major operands, need 268 / 177 registers: no 128 x 128 tiles, two
+// 128 x 64 on a CU: 761 us for a 384-wide model's step, 788 with three and registers in scratch, 784 on 64 x 64) from times measured on pairs of planes, in us: 5 for a tile's start and end, plus per 32 k
 // (n tiles on 256 CUs)                 64 x 64: 0.225, alone on its CU
 //   128 x 128: 0.85 alone, 1.15 for two on a CU             128 x 64: 0.5 alone, 0.75 for two, 1.1 for three.
 // Measured, 64 / 128 for the whole chain of five steps (tiles of 128 in the symmetric products / in P X): 12 x 384^2 (72 / 108) 166 / 236, 16 x 384^2
 // (96 / 144) 251 / 239, 4 x 768^2 (84 / 144) 326 / 354, 12 x 768^2 (252 / 432) 657 / 469, 8 x 384 x 1536 (48 / 288) 277 / 374, 16 x (96 / 576) 493 / 439.
 // 128 x 128 / 128 x 64 for one launch: the four products of twelve 384-wide blocks, Gram 52 / 48, polynomial 27 / 25, P X 63 / 67; 4 x 2048^2, Gram
 // 126 / 121, polynomial 130 / 123, P X 179 / 197; ragged stacks of 192 tiles, P X 15 / 12.
-int tile_kind(const NsTable& t, bool large, bool gram, bool sym, int planes) {
+int tile_kind(const NsTable& t, bool large, bool gram, bool sym, int planes, bool tall) {
     struct Sum { double n = 0., alone = 0., two = 0., three = 0.; } s64, s128, half;
     double n32 = 0.;
     auto add = [](Sum& s, double n, double stages, double alone, double two, double three) {
@@ -954,13 +970,14 @@ int tile_kind(const NsTable& t, bool large, bool gram, bool sym, int planes) {
     const double t64 = ceil(s64.n / 256) * s64.two / s64.n;
     if (!large) return TILE_64;
     const double t128 = s128.n <= 256 ? s128.alone : ceil(s128.n / 512) * s128.two / s128.n;
+    if (gram && planes == 2 && tall) return (half.n <= 256 ? half.alone : fmax(half.alone, fmax(1., half.n / 512) * half.two / half.n)) < t64 ? TILE_HALF : TILE_64;
     const double th = half.n <= 256 ? half.alone : half.n <= 512 ? fmax(half.alone, half.two / half.n) : ceil(half.n / 768) * half.three / half.n;
     return th < t64 && th < t128 ? TILE_HALF : t128 < t64 ? TILE_128 : TILE_64;
 }
 template <int KIND, int PL, int EPI>
 int launch_gemm_v(NsTable& t, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& f, hipStream_t s) {
     using Tile = NsTile<KIND>;
-    const long grid = ns_grid(t, EPI == EPI_GRAM || EPI == EPI_POLY ? TILES_SYM : TILES_MULT, Tile::TR, Tile::TC);
+    const long grid = ns_grid(t, EPI == EPI_GRAM || EPI == EPI_GRAM_ROWS || EPI == EPI_POLY ? TILES_SYM : TILES_MULT, Tile::TR, Tile::TC);
     S3D_REQUIRE(grid >= 0, "newton_schulz: too many tiles");
     auto k = ns_gemm_kernel<KIND, PL, EPI>;
     if (Tile::BYTES > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, Tile::BYTES);
@@ -968,16 +985,28 @@ int launch_gemm_v(NsTable& t, const NsPtrs& p, half_t* ws, const float* hyper, i
     S3D_CHECK_LAUNCH_V("newton_schulz", KIND * 100 + PL * 10 + EPI);
     return 0;
 }
+// planes of the operands (2 or 1) as they occur: results in bf16 come from single planes, fp32 results and the parameters' step from pairs
+template <int EPI> constexpr bool ns_pairs() { return EPI != EPI_OUT_BF16; }
+template <int EPI> constexpr bool ns_single() { return EPI != EPI_OUT_F32 && EPI != EPI_UPDATE; }
 template <int EPI>
 int launch_gemm(NsPlan& pl, int planes, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& f, hipStream_t s) {
-    const int kind = tile_kind(pl.t, pl.pad == 128, EPI == EPI_GRAM, EPI == EPI_GRAM || EPI == EPI_POLY, planes);
-    if (kind == TILE_32) return launch_gemm_v<TILE_32, 2, EPI>(pl.t, p, ws, hyper, which, f, s);
-#define S3D_NS_CASE(k)                                                                                 \
-    if (kind == k) return planes == 2 ? launch_gemm_v<k, 2, EPI>(pl.t, p, ws, hyper, which, f, s)      \
-                                      : launch_gemm_v<k, 1, EPI>(pl.t, p, ws, hyper, which, f, s);
-    S3D_NS_CASE(TILE_128) S3D_NS_CASE(TILE_HALF)
-#undef S3D_NS_CASE
-    return planes == 2 ? launch_gemm_v<TILE_64, 2, EPI>(pl.t, p, ws, hyper, which, f, s) : launch_gemm_v<TILE_64, 1, EPI>(pl.t, p, ws, hyper, which, f, s);
+    bool tall = false;
+    for (int i = 0; i < pl.t.n; ++i) tall |= pl.t.d[i].tall != 0;
+    const int kind = tile_kind(pl.t, pl.pad == 128, EPI == EPI_GRAM, EPI == EPI_GRAM || EPI == EPI_POLY, planes, tall);
+    constexpr int ROWS = EPI == EPI_GRAM ? EPI_GRAM_ROWS : EPI;
+    if constexpr (ns_pairs<EPI>()) {
+        if (planes == 2) {
+            if (kind == TILE_32) return launch_gemm_v<TILE_32, 2, EPI>(pl.t, p, ws, hyper, which, f, s);
+            if (kind == TILE_64) return launch_gemm_v<TILE_64, 2, EPI>(pl.t, p, ws, hyper, which, f, s);
+            if (kind == TILE_128) return launch_gemm_v<TILE_128, 2, ROWS>(pl.t, p, ws, hyper, which, f, s);
+            return tall ? launch_gemm_v<TILE_HALF, 2, EPI>(pl.t, p, ws, hyper, which, f, s) : launch_gemm_v<TILE_HALF, 2, ROWS>(pl.t, p, ws, hyper, which, f, s);
+        }
+    }
+    if constexpr (ns_single<EPI>()) {
+        if (planes == 1) return kind == TILE_64 ? launch_gemm_v<TILE_64, 1, EPI>(pl.t, p, ws, hyper, which, f, s)
+                              : kind == TILE_128 ? launch_gemm_v<TILE_128, 1, EPI>(pl.t, p, ws, hyper, which, f, s) : launch_gemm_v<TILE_HALF, 1, EPI>(pl.t, p, ws, hyper, which, f, s);
+    }
+    S3D_REQUIRE(false, "newton_schulz: no kernel for %d planes", planes);
 }
 
 // Polynomial and P X in one launch?  Sides that fit, tiles of P X on the CUs once over.  Whole call, two launches / one, us: 192 x 192 93 / 76, the
@@ -991,15 +1020,21 @@ bool small_sides(const NsTable& t) {
     }
     return n <= 256;
 }
-template <int PL, int EPI>
-int launch_small(NsPlan& pl, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& poly, const NsScale& mult, hipStream_t s) {
+template <int EPI>
+int launch_small(NsPlan& pl, int planes, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& poly, const NsScale& mult, hipStream_t s) {
     const long grid = ns_grid(pl.t, TILES_MULT);
     S3D_REQUIRE(grid >= 0, "newton_schulz: too many tiles");
-    auto k = ns_small_kernel<PL, EPI>;
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_BYTES);
-    hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(512), SMALL_BYTES, s, pl.t, p, ws, hyper, which, poly, mult);
-    S3D_CHECK_LAUNCH_V("newton_schulz_small", PL * 10 + EPI);
-    return 0;
+    auto run = [&](auto k) {
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_BYTES);
+        hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(512), SMALL_BYTES, s, pl.t, p, ws, hyper, which, poly, mult);
+        S3D_CHECK_LAUNCH_V("newton_schulz_small", planes * 10 + EPI);
+        return 0;
+    };
+    if constexpr (ns_pairs<EPI>())
+        if (planes == 2) return run(ns_small_kernel<2, EPI>);
+    if constexpr (ns_single<EPI>())
+        if (planes == 1) return run(ns_small_kernel<1, EPI>);
+    S3D_REQUIRE(false, "newton_schulz: no kernel for %d planes", planes);
 }
 
 template <int SRC, int LAST>
@@ -1035,8 +1070,7 @@ int ns_run(NsPlan& pl, const NsPtrs& p, const S3dNsArgs& a, const float* hyper, 
         const bool end = k + 1 == a.steps;
         int rc;
         if (small) {
-            if (planes == 2) rc = end ? launch_small<2, LAST>(pl, p, ws, hyper, k & 1, poly, last, s) : launch_small<2, EPI_MULT>(pl, p, ws, hyper, k & 1, poly, mult, s);
-            else rc = end ? launch_small<1, LAST>(pl, p, ws, hyper, k & 1, poly, last, s) : launch_small<1, EPI_MULT>(pl, p, ws, hyper, k & 1, poly, mult, s);
+            rc = end ? launch_small<LAST>(pl, planes, p, ws, hyper, k & 1, poly, last, s) : launch_small<EPI_MULT>(pl, planes, p, ws, hyper, k & 1, poly, mult, s);
         } else {
             rc = launch_gemm<EPI_POLY>(pl, planes, p, ws, hyper, k & 1, poly, s);
             if (!rc) rc = end ? launch_gemm<LAST>(pl, planes, p, ws, hyper, k & 1, last, s) : launch_gemm<EPI_MULT>(pl, planes, p, ws, hyper, k & 1, mult, s);
