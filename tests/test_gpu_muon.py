@@ -48,7 +48,7 @@ def grads(L, r, c, seed=0, dtype=torch.float32):
 SHAPES = [(1, 1, 1), (2, 1, 7), (2, 9, 1), (3, 5, 3), (1, 16, 16), (1, 64, 64), (2, 65, 64), (1, 63, 130), (2, 130, 63), (1, 192, 192), (2, 192, 576), (2, 576, 192),
           (1, 387, 1000), (1, 1000, 387), (3, 384, 384), (1, 768, 768), (1, 2, 5000), (1, 1031, 129), (5, 128, 256), (1, 129, 257), (2, 500, 100), (3, 90, 100),
           # enough tiles for the large ones: wide, tall, square, padded
-          (12, 384, 1536), (12, 1536, 384), (2, 1536, 1530), (2, 1500, 1600), (9, 700, 640), (30, 250, 384)]
+          (12, 384, 1536), (12, 1536, 384), (2, 1536, 1530), (2, 1500, 1600), (9, 700, 640), (30, 250, 384), (130, 256, 520), (130, 520, 256)]
 
 
 @pytest.mark.parametrize('L,r,c', SHAPES)
