@@ -1182,6 +1182,7 @@ int s3d_launch_orthogonalize(const S3dOrthoItem* items, int n, const S3dNsArgs* 
         S3D_REQUIRE(q.x_ld >= q.cols && q.out_ld >= q.cols, "%s: item %d: row pitch below %d columns", who, i, q.cols);
         S3D_REQUIRE(q.count == 1 || q.out_stride >= (long)(q.rows - 1) * q.out_ld + q.cols, "%s: item %d: output matrices overlap", who, i);
     }
+    if (n == 0) return 0;
     const size_t need = ns_workspace(items, n);
     S3D_REQUIRE(workspace && bytes >= need && ((uintptr_t)workspace & 15) == 0, "%s: the workspace needs %zu bytes, 16-byte aligned", who, need);
     NsRanges used(2L * n);
@@ -1223,6 +1224,7 @@ int s3d_launch_muon(const S3dMuonItem* items, int n, const S3dNsArgs* a, const f
                     "%s: item %d: matrices of the stack overlap", who, i);
         S3D_REQUIRE(isfinite(q.scale), "%s: item %d: non-finite scale", who, i);
     }
+    if (n == 0) return 0;
     const size_t need = ns_workspace(items, n);
     S3D_REQUIRE(workspace && bytes >= need && ((uintptr_t)workspace & 15) == 0, "%s: the workspace needs %zu bytes, 16-byte aligned", who, need);
     NsRanges used(5L * n);

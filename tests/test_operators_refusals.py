@@ -185,3 +185,11 @@ def test_muon_refuses_one_gradient_for_two_parameters_when_it_is_cleared(lib):
 def test_orthogonalize_refuses_shared_outputs(lib, second):
     f = [dict(dict(x=A, out=2 * A), **kw) for kw in ({}, second)]
     refused(lib.s3d_orthogonalize(items(L.S3dOrthoItem, ortho, *f), 2, ns(), P, 1 << 40, None), lib, 'shares memory')
+
+
+def test_no_items_are_no_work(lib):
+    """An empty list needs no workspace: what the size calls say (0) is enough."""
+    assert lib.s3d_muon_workspace_bytes(None, 0, ns()) == 0 and lib.s3d_orthogonalize_workspace_bytes(None, 0, ns()) == 0
+    assert lib.s3d_muon_step(None, 0, ns(), P, None, 0, None) == 0
+    assert lib.s3d_orthogonalize(None, 0, ns(), None, 0, None) == 0
+    refused(lib.s3d_muon_step(None, 0, ns(steps=0), P, None, 0, None), lib, 'steps')
