@@ -335,3 +335,25 @@ def test_muon_step_over_small_sides(shapes, zero):
         hi = p[i].bfloat16()
         assert torch.equal(planes[i][0], hi) and torch.equal(planes[i][1], (p[i] - hi.float()).bfloat16())
         assert torch.equal(gr[i], torch.zeros_like(gr[i]) if zero else g0[i])
+
+
+def test_stacks_whose_offsets_pass_32_bits():
+    """matrices 1.2 10^9 elements apart, and a workspace of more than 2^32 bytes: the results of compact stacks, bit for bit"""
+    stride, r, c = 1_200_000_000, 70, 150
+    buf = torch.empty(2 * stride + r * c, device=DEV)
+    far = buf.as_strided((3, r, c), (stride, c, 1))
+    g, m, p = (grads(3, r, c, seed=s) for s in range(3))
+    far.copy_(p)
+    hyper = torch.tensor([0.02, 0.9, 0.1, 1.0], device=DEV)
+    m2 = m.clone()
+    ops.muon_step([far], [g], [m2], hyper)
+    ops.muon_step([p], [g], [m], hyper)
+    assert torch.equal(far, p) and torch.equal(m, m2)
+    far.copy_(g)
+    assert torch.equal(ops.orthogonalize(far, out=far), ops.orthogonalize(g))
+    del buf, far
+    many = grads(1, 192, 192).expand(20000, 192, 192)
+    out = ops.orthogonalize(many)
+    few = ops.orthogonalize(many[:40].contiguous())                  # (fewer matrices take other tiles: the tolerance of two results)
+    assert torch.equal(out[0], out[-1]) and torch.equal(out[0], out[9999])
+    assert rel(out[-1:], few[:1]) <= 2 * tol(5)
