@@ -248,7 +248,7 @@ int lanes_of(int hd) {
 }
 // Rows of one workgroup: one pass of its groups over the heads while there are few rows, about 2048 row ranges (x 3 roles) when there are many.
 // Backward: a workgroup ends by adding its groups' gain gradients through LDS, and every row range is a row of the reduction behind it, so up to four
-// passes as long as 900 workgroups are left.  One / two / four passes, us with the reduction: 1203 ranges of 128-wide heads 23.4 / 17.7 / 16.7,
+// passes as long as 900 workgroups are left.  One / two / four passes, us with the reduction: 1203 ranges of 80-wide heads 23.4 / 17.7 / 16.7,
 // 747 ranges of 64-wide heads 19.6 / 16.6 / 17.3.
 int rows_per_wg(long rows, int H, int hd, bool bwd) {
     const int groups = 256 / lanes_of(hd);
