@@ -421,7 +421,8 @@ int s3d_adam_step_wire(float* p, float* g, const uint16_t* g_wire, float* m, flo
  * Newton-Schulz: X0 = U / max(|U|_F, eps), then `steps` times  A = X X^T,  X <- a X + (b A + c A^2) X  (a tall matrix:
  * A = X^T X, from the right): every singular value s becomes a s + b s^3 + c s^5, the singular vectors stay.  A stack item is `count` matrices
  * [rows][cols] of one shape: matrix i of a tensor at + i * stride, row pitch ld (elements); any sizes, no alignment beyond the element's;
- * items with a zero size are skipped.  Products are taken on pairs of fp16 planes with fp32 accumulation (fp32-class, csrc/muon.hip).
+ * items with a zero size are skipped.  Products are taken on pairs of fp16 planes with fp32 accumulation (fp32-class, csrc/muon.hip); a bf16 result is
+ * the fp32 result rounded once.
  * Non-finite entries make that matrix's result NaN.  Calls are bitwise reproducible.  Tensors that are written may share no element with another item's
  * (blocks of one matrix and matrices interleaved in one arena are told apart; other overlapping layouts are refused).
  * workspace: device scratch of at least the size the *_workspace_bytes call gives for the SAME items (16-byte aligned; contents are

@@ -13,7 +13,8 @@
 // (hi = rne(x s), lo = rne(x s - hi), 22 bits; s a power of two that keeps the largest possible entry below 2^15) multiplied as
 // hi lo + lo hi + hi hi with fp32 accumulation: an fp32 product at a third of the fp16 matrix rate, five times that of the fp32 matrix
 // instructions.  fp16 planes rather than bf16: all entries are bounded by the spectral norm, so the exponent range is not needed and
-// the six extra bits are.
+// the six extra bits are.  Results in bf16 take the same products and are rounded once, at the end: the last two steps on the hi planes alone would save
+// a fifth of 4 x 2048^2 (2110 us to 1646) and cost up to another rounding of the result (2 * 2^-12 (a^2 + a): 0.7 % for a = 3.44, more for a larger a).
 //
 // Bound: the matrix cores for large stacks (4 x 2048^2: P X 161 - 200 us = 1030 - 1280 TF of fp16 products, a large library product 1095), the balance of uneven
 // k over the CUs for a model's (48 matrices, 384 wide: Gram 48 us of 30, P X 63 of 45, the last product HBM: 425 MB in 87 us), what one CU can fetch and
@@ -92,10 +93,9 @@ __device__ __forceinline__ long off_x(const NsDims& d, int which) { return 2L * 
 __device__ __forceinline__ long off_a(const NsDims& d) { return 4L * d.rp * d.cp; }
 __device__ __forceinline__ long off_p(const NsDims& d) { return 4L * d.rp * d.cp + 2L * d.mp * d.mp; }
 
-// Planes in memory.  A pair is stored in blocks of 32 columns, [hi 32 | lo 32] = one 128-byte line: a stage of 32 k of a row is ONE line (with two
-// separate planes every line was fetched twice, half of it each time: 12 TB/s of useful L2 traffic instead of 20).  A single plane is plain row
-// major, a stage is then 64 k and again one line per row.
-__device__ __forceinline__ long ns_at(bool pair, long r, int c, int ld) { return pair ? r * 2 * ld + ((c >> 5) << 6) + (c & 31) : r * ld + c; }
+// Pairs in memory: blocks of 32 columns, [hi 32 | lo 32] = one 128-byte line, so that a stage of 32 k of a row is ONE line (with two separate planes
+// every line was fetched twice, half of it each time: 12 TB/s of useful L2 traffic instead of 20).
+__device__ __forceinline__ long ns_at(long r, int c, int ld) { return r * 2 * ld + ((c >> 5) << 6) + (c & 31); }
 
 __device__ __forceinline__ void split_half(float v, half_t& hi, half_t& lo) {
     hi = (half_t)v;
@@ -196,10 +196,10 @@ __global__ __launch_bounds__(256) void ns_sumsq_kernel(const NsTable t, const Ns
     if (threadIdx.x == 0) part[d.part + (long)mat * d.chunks + chunk] = red[0];
 }
 
-// ---- 2. X0 = U / max(|U|, eps) as planes, padding cleared: 2048 elements of [rp][cp] per workgroup ----
+// ---- 2. X0 = U / max(|U|, eps) as pairs, padding cleared: 2048 elements of [rp][cp] per workgroup ----
 template <int SRC>
 __global__ __launch_bounds__(256) void ns_load_kernel(const NsTable t, const NsPtrs p, const float* __restrict__ hyper, int nesterov,
-                                                      const double* __restrict__ part, float eps, float sx, int pair, half_t* __restrict__ ws) {
+                                                      const double* __restrict__ part, float eps, float sx, half_t* __restrict__ ws) {
     NsPlace w;
     if (!ns_place(t, w)) return;
     const int it = w.it, mat = w.mat, blk = w.tile;
@@ -246,9 +246,9 @@ __global__ __launch_bounds__(256) void ns_load_kernel(const NsTable t, const NsP
         h[i] = a;
         l[i] = b;
     }
-    half_t* X = ws + d.ws + mat * d.wsz + ns_at(pair, r, c, d.cp);
+    half_t* X = ws + d.ws + mat * d.wsz + ns_at(r, c, d.cp);
     *reinterpret_cast<half8*>(X) = h;
-    if (pair) *reinterpret_cast<half8*>(X + 32) = l;
+    *reinterpret_cast<half8*>(X + 32) = l;
 }
 
 // ---- 3. the products ----
@@ -256,36 +256,36 @@ __global__ __launch_bounds__(256) void ns_load_kernel(const NsTable t, const NsP
 // the tile starts at i = at.
 struct NsOperand { const half_t* p; int ld, at; };
 
-// One stage of an operand is T x 128 bytes of LDS: T rows of one line (k-contiguous), or 32 (pairs) / 64 k rows of the tile's columns (k-major).
+// One stage of an operand is T x 128 bytes of LDS: T rows of one line (k-contiguous), or 32 k rows of the tile's columns (k-major).
 // Piece q of it is 1 KB = one DMA instruction of a wave; every lane brings 16 bytes, the slot swizzle is applied here.  A lane's byte offset from ns_base is
 // (ns_lane_source ^ ns_flip(q)) + q * rows of a piece * row: the swizzles are linear in the row's bits and a row is a multiple of what they permute, so a
 // wave keeps one register for all its pieces.
-template <int T, int PL, bool KM>
+template <int T, bool KM>
 struct NsPieces {
-    static constexpr int W = PL * T, WK = W / 8;                     // k-major: halves / 16-byte slots of a row
+    static constexpr int W = 2 * T, WK = W / 8;                     // k-major: halves / 16-byte slots of a row
     static constexpr int ROWS = KM ? 64 / WK : 8;                    // of a piece
 };
-template <int T, int PL, bool KM>
+template <int T, bool KM>
 __device__ __forceinline__ unsigned ns_lane_source(const NsOperand& o, int lane) {
-    using P = NsPieces<T, PL, KM>;
+    using P = NsPieces<T, KM>;
     const int r = KM ? lane / P::WK : lane >> 3, chunk = KM ? (lane % P::WK) ^ kmajor_swz<P::W>(r) : (lane & 7) ^ dma_swz64(r);
-    return (unsigned)(r * PL * o.ld + chunk * 8) * 2;
+    return (unsigned)(r * 2 * o.ld + chunk * 8) * 2;
 }
-template <int T, int PL, bool KM>
+template <int T, bool KM>
 __device__ __forceinline__ unsigned ns_flip(int piece) {
-    using P = NsPieces<T, PL, KM>;
+    using P = NsPieces<T, KM>;
     return (KM ? kmajor_swz<P::W>(piece * P::ROWS) : dma_swz64(piece * P::ROWS)) * 16;
 }
-template <int T, int PL, bool KM>
-__device__ __forceinline__ int ns_advance(const NsOperand& o, int piece) { return piece * NsPieces<T, PL, KM>::ROWS * PL * o.ld; }      // in halves
-template <int T, int PL, bool KM>
+template <int T, bool KM>
+__device__ __forceinline__ int ns_advance(const NsOperand& o, int piece) { return piece * NsPieces<T, KM>::ROWS * 2 * o.ld; }      // in halves
+template <int T, bool KM>
 __device__ __forceinline__ unsigned ns_source(const NsOperand& o, int piece, int lane) {           // (at most 192 rows)
-    return (ns_lane_source<T, PL, KM>(o, lane) ^ ns_flip<T, PL, KM>(piece)) + (unsigned)ns_advance<T, PL, KM>(o, piece) * 2;
+    return (ns_lane_source<T, KM>(o, lane) ^ ns_flip<T, KM>(piece)) + (unsigned)ns_advance<T, KM>(o, piece) * 2;
 }
-template <int PL, bool KM>
-__device__ __forceinline__ const half_t* ns_base(const NsOperand& o) { return o.p + (KM ? (long)o.at * PL : (long)o.at * PL * o.ld); }
-template <int PL, bool KM>
-__device__ __forceinline__ long ns_step(const NsOperand& o) { return KM ? 64L * o.ld : 64; }      // halves from stage to stage (32 rows of 2 ld, or 64 rows of ld)
+template <bool KM>
+__device__ __forceinline__ const half_t* ns_base(const NsOperand& o) { return o.p + (KM ? 2L * o.at : 2L * o.at * o.ld); }
+template <bool KM>
+__device__ __forceinline__ long ns_step(const NsOperand& o) { return KM ? 64L * o.ld : 64; }      // halves from stage to stage (32 rows of 2 ld, or one line)
 // one piece: every lane's 16 bytes at base + off land lane-linear at LDS byte address dst (all but off wave-uniform).  The compiler does not count the
 // load: it is retired with a counted wait before anything reads the piece.
 __device__ __forceinline__ void ns_dma(const half_t* base, unsigned off, unsigned dst) {
@@ -309,16 +309,16 @@ __device__ __forceinline__ void ns_barrier() {
 }
 
 // A lane's LDS address of the fragments whose rows / columns begin at w0 (a multiple of 32, of 16 for a single one), of an operand's tile at `tile`
-// (a multiple of 512); fragment (q, i), rows / columns w0 + 16 i .. + 15, is a constant away: q = plane (pairs), or which half of the stage's 64 k.  Both
+// (a multiple of 512); fragment (q, i), plane q of rows / columns w0 + 16 i .. + 15, is a constant away.  Both
 // swizzles depend on the lane alone, so that one register per operand is kept instead of one per fragment.
-template <int T, int PL, bool KM>
+template <int T, bool KM>
 __device__ __forceinline__ unsigned ns_lane(const unsigned char* tile, int w0, int lane) {
     if constexpr (!KM) {
         const int r = w0 + (lane & 15);
         return (unsigned)(uintptr_t)tile + r * 128 + (((lane >> 4) ^ dma_swz64(r)) << 4);
-    } else return kmajor_addr<PL * T>(tile, PL == 2 ? (w0 >> 5) * 64 + (w0 & 31) : w0, (lane >> 4) * 8, lane);
+    } else return kmajor_addr<2 * T>(tile, (w0 >> 5) * 64 + (w0 & 31), (lane >> 4) * 8, lane);
 }
-template <int T, int PL, bool KM>
+template <int T, bool KM>
 __device__ __forceinline__ half8 ns_frag(unsigned at, int q, int i) {
     if constexpr (!KM) {
         typedef __attribute__((address_space(3))) half8 lds_half8;
@@ -326,9 +326,9 @@ __device__ __forceinline__ half8 ns_frag(unsigned at, int q, int i) {
     } else {
         typedef __attribute__((ext_vector_type(4))) short short4v;
         typedef __attribute__((address_space(3))) short4v lds_short4;
-        constexpr int ROW = PL * T * 2;                                              // bytes
+        constexpr int ROW = 4 * T;                                                   // bytes
         struct { short4v a, b; } u;
-        const unsigned ad = PL == 2 ? at ^ ((i >> 1) * 128 + q * 64 + (i & 1) * 32) : (at ^ (i * 32)) + q * 32 * ROW;
+        const unsigned ad = at ^ ((i >> 1) * 128 + q * 64 + (i & 1) * 32);
         u.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)ad);
         u.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)(ad + 4 * ROW));
         return __builtin_bit_cast(half8, u);
@@ -336,22 +336,20 @@ __device__ __forceinline__ half8 ns_frag(unsigned at, int q, int i) {
 }
 template <int FR, int FC>
 struct NsFrags { half8 l[2][FR], r[2][FC]; };
-// the fragments of a stage, and the products [from, to) of its 3 FR FC (pairs: hi lo, lo hi, hi hi) or 2 FR FC (the two halves of a single-plane
-// stage): numbered so that they can be dealt out between the other instructions of a stage
-template <int T, int F, int PL, bool KM>
+// the fragments of a stage, and the products [from, to) of its 3 FR FC (hi lo, lo hi, hi hi): numbered so that they can be dealt out between the other
+// instructions of a stage
+template <int T, int F, bool KM>
 __device__ __forceinline__ void ns_read(half8 (&f)[2][F], unsigned at) {
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int i = 0; i < F; ++i) f[q][i] = ns_frag<T, PL, KM>(at, q, i);
+        for (int i = 0; i < F; ++i) f[q][i] = ns_frag<T, KM>(at, q, i);
 }
-template <int PL, int FR, int FC>
-constexpr int ns_products() { return (PL == 2 ? 3 : 2) * FR * FC; }
 // Sums of a tile.  The matrix cores' accumulation rounds towards zero at the size of what is there, so one running sum of three products per 32 k is
 // off to one side, for all singular values together (results of orthogonalize 1.1e-6 .. 2.3e-6 off in the 2-norm; 0.5e-6 .. 0.7e-6 with these and the shift of A below).
 // SPLIT (the short sums of a wave that has a part of k): hi hi in one sum, the two products 2^11 smaller in another.  Else: two stages begin at zero,
-// small products first, and are added to a total that rounds to nearest.  (Single planes: one sum.)
-template <int FR, int FC, int PL, bool SPLIT>
+// small products first, and are added to a total that rounds to nearest.
+template <int FR, int FC, bool SPLIT>
 struct NsSums {
     f32x4 sum[FR][FC], more[FR][FC];
     __device__ __forceinline__ void clear() {
@@ -361,7 +359,7 @@ struct NsSums {
             for (int j = 0; j < FC; ++j) sum[i][j] = more[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     __device__ __forceinline__ void flush() {
-        if constexpr (PL == 2 && !SPLIT) {
+        if constexpr (!SPLIT) {
 #pragma unroll
             for (int i = 0; i < FR; ++i)
 #pragma unroll
@@ -369,48 +367,46 @@ struct NsSums {
         }
     }
     __device__ __forceinline__ f32x4 get(int i, int j) const {
-        if constexpr (PL == 1) return sum[i][j];
-        else if constexpr (SPLIT) return sum[i][j] + more[i][j];
+        if constexpr (SPLIT) return sum[i][j] + more[i][j];
         else return more[i][j];
     }
 };
 // FIRST: the first of two stages
-template <bool FIRST, int FR, int FC, int PL, bool SPLIT>
-__device__ __forceinline__ void ns_mfma(const NsFrags<FR, FC>& f, NsSums<FR, FC, PL, SPLIT>& acc, int from = 0, int to = ns_products<PL, FR, FC>()) {
+template <bool FIRST, int FR, int FC, bool SPLIT>
+__device__ __forceinline__ void ns_mfma(const NsFrags<FR, FC>& f, NsSums<FR, FC, SPLIT>& acc, int from = 0, int to = 3 * FR * FC) {
 #pragma unroll
     for (int e = from; e < to; ++e) {
-        const int q = e / (FR * FC), i = e / FC % FR, j = e % FC, ql = PL == 2 ? q == 1 : q, qr = PL == 2 ? q == 0 : q;
-        f32x4& a = SPLIT && PL == 2 && q < 2 ? acc.more[i][j] : acc.sum[i][j];
-        const f32x4 c = !SPLIT && FIRST && PL == 2 && q == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : a;
+        const int q = e / (FR * FC), i = e / FC % FR, j = e % FC, ql = q == 1, qr = q == 0;
+        f32x4& a = SPLIT && q < 2 ? acc.more[i][j] : acc.sum[i][j];
+        const f32x4 c = !SPLIT && FIRST && q == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : a;
         a = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.r[qr][j], f.l[ql][i], c, 0, 0, 0);
     }
 }
 
 // acc = sum over k of L(i, k) R(j, k) for a TR x TC tile by 2 x 2 waves of TR/2 x TC/2: a ring of
 // RING stages filled by LDS-DMA; the fragments of the next stage are read while the matrix cores work on this one (a SIMD has
-// two waves: without that the LDS time of a stage adds to its MFMA time).  PL planes (2: hi lo + lo hi + hi hi; stages of 32 k.  1: stages of
-// 64 k).  K is a multiple of 64.  acc.get(i, j)[e] = C[wr + 16 i + (lane & 15)][wc + 16 j + 4 (lane >> 4) + e].
-template <int TR, int TC, int RING, int PL, bool LK, bool RK>
-__device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& R, int K, unsigned char* smem, NsSums<TR / 32, TC / 32, PL, false>& acc) {
+// two waves: without that the LDS time of a stage adds to its MFMA time).  K is a multiple of 64, a stage 32 of it.  acc.get(i, j)[e] = C[wr + 16 i + (lane & 15)][wc + 16 j + 4 (lane >> 4) + e].
+template <int TR, int TC, int RING, bool LK, bool RK>
+__device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& R, int K, unsigned char* smem, NsSums<TR / 32, TC / 32, false>& acc) {
     constexpr int STAGE = (TR + TC) * 128;                           // bytes: L, R
     constexpr int PIECES = STAGE / 1024 / 4;                         // 1 KB DMA pieces per wave and stage: wave w brings w PIECES .. of L's and R's
     constexpr int LEFT = TR / 8, FR = TR / 32, FC = TC / 32;         // L's pieces; 16-row fragments per wave
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int left = LEFT - wave * PIECES;                           // this wave's pieces below `left` are L's
-    const long step_l = ns_step<PL, LK>(L), step_r = ns_step<PL, RK>(R);
-    const half_t *src_l = ns_base<PL, LK>(L), *src_r = ns_base<PL, RK>(R);
-    const unsigned off_l = ns_lane_source<TR, PL, LK>(L, lane), off_r = ns_lane_source<TC, PL, RK>(R, lane);
+    const long step_l = ns_step<LK>(L), step_r = ns_step<RK>(R);
+    const half_t *src_l = ns_base<LK>(L), *src_r = ns_base<RK>(R);
+    const unsigned off_l = ns_lane_source<TR, LK>(L, lane), off_r = ns_lane_source<TC, RK>(R, lane);
     auto bring = [&](unsigned at) {                                  // this wave's pieces of the next stage
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             const int ql = wave * PIECES + i, qr = ql - LEFT;
-            const half_t* src = i < left ? src_l + ns_advance<TR, PL, LK>(L, ql) : src_r + ns_advance<TC, PL, RK>(R, qr);
-            const unsigned off = i < left ? off_l ^ ns_flip<TR, PL, LK>(ql) : off_r ^ ns_flip<TC, PL, RK>(qr);
+            const half_t* src = i < left ? src_l + ns_advance<TR, LK>(L, ql) : src_r + ns_advance<TC, RK>(R, qr);
+            const unsigned off = i < left ? off_l ^ ns_flip<TR, LK>(ql) : off_r ^ ns_flip<TC, RK>(qr);
             ns_dma(src, off, at + i * 1024);
         }
     };
     const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)smem + wave * PIECES * 1024);
-    const int KT = K / (PL == 2 ? 32 : 64);
+    const int KT = K / 32;
     unsigned slot_in = 0, slot = 0;                                  // in bytes
     auto advance = [](unsigned& s) { s = s == (RING - 1) * STAGE ? 0 : s + STAGE; };
     acc.clear();
@@ -426,9 +422,9 @@ __device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& 
     else ns_wait<0, false>();
     ns_barrier();
     NsFrags<FR, FC> fa, fb;
-    const unsigned lane_l = ns_lane<TR, PL, LK>(smem, wr, lane), lane_r = ns_lane<TC, PL, RK>(smem + TR * 128, wc, lane);
-    ns_read<TR, FR, PL, LK>(fa.l, lane_l);
-    ns_read<TC, FC, PL, RK>(fa.r, lane_r);
+    const unsigned lane_l = ns_lane<TR, LK>(smem, wr, lane), lane_r = ns_lane<TC, RK>(smem + TR * 128, wc, lane);
+    ns_read<TR, FR, LK>(fa.l, lane_l);
+    ns_read<TC, FC, RK>(fa.r, lane_r);
     auto body = [&](auto first, int kt, NsFrags<FR, FC>& now, NsFrags<FR, FC>& next) {
         constexpr bool FIRST = decltype(first)::value;
         // this wave holds stage kt in registers (lgkmcnt) and its pieces of stage kt + 1 have landed; behind the barrier that is true of every wave:
@@ -439,12 +435,12 @@ __device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& 
         const bool more = kt + RING < KT;
         advance(slot);
         // the reads lie under the products (finer interleavings of loads, reads and products measured the same or slower)
-        constexpr int M = ns_products<PL, FR, FC>();
+        constexpr int M = 3 * FR * FC;
         if (more) bring(lds0 + slot_in);
         ns_mfma<FIRST>(now, acc, 0, M / 3);
-        ns_read<TR, FR, PL, LK>(next.l, lane_l + slot);
+        ns_read<TR, FR, LK>(next.l, lane_l + slot);
         ns_mfma<FIRST>(now, acc, M / 3, 2 * M / 3);
-        ns_read<TC, FC, PL, RK>(next.r, lane_r + slot);              // (lo of either side is done: all at once are 32 registers more)
+        ns_read<TC, FC, RK>(next.r, lane_r + slot);              // (lo of either side is done: all at once are 32 registers more)
         ns_mfma<FIRST>(now, acc, 2 * M / 3, M);
         src_l += step_l;
         src_r += step_r;
@@ -461,18 +457,18 @@ __device__ __forceinline__ void ns_product(const NsOperand& L, const NsOperand& 
 // stages, brought by itself, so nothing is waited for but its own loads; a quarter of the serial length and half the LDS reads per product.  The
 // four partial sums are added through LDS in the order of the waves.  64: out[j][e] = C[16 wave + (lane & 15)][16 j + 4 (lane >> 4) + e]; 32: out[0][e] =
 // C[16 (wave >> 1) + (lane & 15)][16 (wave & 1) + 4 (lane >> 4) + e].
-template <int T, int RING, int PL, bool LK, bool RK>
+template <int T, int RING, bool LK, bool RK>
 __device__ __forceinline__ void ns_product_ksplit(const NsOperand& L, const NsOperand& R, int K, unsigned char* smem, f32x4 (&out)[T * T / 1024]) {
     constexpr int STAGE = 2 * T * 128, PIECES = STAGE / 1024, F = T / 16, MINE = F * F / 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     unsigned char* mine = smem + wave * RING * STAGE;
     const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)mine);
-    const int KT = (K / (PL == 2 ? 32 : 64) - wave + 3) / 4;         // stages wave, wave + 4, ..
-    const long step_l = ns_step<PL, LK>(L), step_r = ns_step<PL, RK>(R);
-    const half_t *src_l = ns_base<PL, LK>(L) + wave * step_l, *src_r = ns_base<PL, RK>(R) + wave * step_r;
+    const int KT = (K / 32 - wave + 3) / 4;         // stages wave, wave + 4, ..
+    const long step_l = ns_step<LK>(L), step_r = ns_step<RK>(R);
+    const half_t *src_l = ns_base<LK>(L) + wave * step_l, *src_r = ns_base<RK>(R) + wave * step_r;
     unsigned off[PIECES];
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) off[i] = i >= PIECES / 2 ? ns_source<T, PL, RK>(R, i - PIECES / 2, lane) : ns_source<T, PL, LK>(L, i, lane);
+    for (int i = 0; i < PIECES; ++i) off[i] = i >= PIECES / 2 ? ns_source<T, RK>(R, i - PIECES / 2, lane) : ns_source<T, LK>(L, i, lane);
     unsigned slot = 0;                                               // in bytes
     auto issue = [&](unsigned at) {
 #pragma unroll
@@ -480,16 +476,16 @@ __device__ __forceinline__ void ns_product_ksplit(const NsOperand& L, const NsOp
         src_l += 4 * step_l;
         src_r += 4 * step_r;
     };
-    NsSums<F, F, PL, true> acc;
+    NsSums<F, F, true> acc;
     acc.clear();
-    const unsigned lane_l = ns_lane<T, PL, LK>(mine, 0, lane), lane_r = ns_lane<T, PL, RK>(mine + T * 128, 0, lane);
+    const unsigned lane_l = ns_lane<T, LK>(mine, 0, lane), lane_r = ns_lane<T, RK>(mine + T * 128, 0, lane);
     for (int k = 0; k < RING && k < KT; ++k) issue(k * STAGE);
     for (int kt = 0; kt < KT; ++kt) {
         if (kt + RING <= KT) ns_wait<(RING - 1) * PIECES, false>();
         else ns_wait<0, false>();
         NsFrags<F, F> f;
-        ns_read<T, F, PL, LK>(f.l, lane_l + slot);
-        ns_read<T, F, PL, RK>(f.r, lane_r + slot);
+        ns_read<T, F, LK>(f.l, lane_l + slot);
+        ns_read<T, F, RK>(f.r, lane_r + slot);
         ns_wait<63, true>();                                         // the slot is in registers: refill it
         if (kt + RING < KT) issue(slot);
         slot = slot == (RING - 1) * STAGE ? 0 : slot + STAGE;
@@ -513,7 +509,7 @@ __device__ __forceinline__ void ns_product_ksplit(const NsOperand& L, const NsOp
 
 // How a tile is worked.  TILE_128: 128 x 128, four waves, 66 KB of LDS: two workgroups share a CU, one's start and epilogue lie under the other's
 // products.  TILE_HALF: 128 x 64, 48 KB, three on a CU: half the granularity for half again the LDS traffic per product.  TILE_64: 64 x 64, the
-// k range over the four waves: launches with too few tiles for the CUs.  TILE_32 the same with 32 x 32 (pairs), 70 KB, two on a CU: launches with so few that
+// k range over the four waves: launches with too few tiles for the CUs.  TILE_32 the same with 32 x 32, 70 KB, two on a CU: launches with so few that
 // what one CU can fetch is the bound.
 enum { TILE_128 = 0, TILE_64 = 1, TILE_HALF = 2, TILE_32 = 3 };
 template <int KIND>
@@ -527,14 +523,14 @@ struct NsTile {
     static constexpr int BYTES = KSPLIT ? RING_BYTES + SUM_BYTES : SUM_BYTES > RING_BYTES ? SUM_BYTES : RING_BYTES;
 };
 
-// 8 elements of a tensor of the iteration at column c (a multiple of 8), stored as a pair or as one plane
-__device__ __forceinline__ void ns_store8(half_t* base, bool pair, long r, int c, int ld, const float* v) {
+// 8 elements of a tensor of the iteration at column c (a multiple of 8)
+__device__ __forceinline__ void ns_store8(half_t* base, long r, int c, int ld, const float* v) {
     half8 h, l;
 #pragma unroll
     for (int e = 0; e < 8; ++e) { half_t a, b; split_half(v[e], a, b); h[e] = a; l[e] = b; }
-    half_t* o = base + ns_at(pair, r, c, ld);
+    half_t* o = base + ns_at(r, c, ld);
     *reinterpret_cast<half8*>(o) = h;
-    if (pair) *reinterpret_cast<half8*>(o + 32) = l;
+    *reinterpret_cast<half8*>(o + 32) = l;
 }
 
 // the last product's epilogue for n <= 8 elements of a row: the result, or the parameters' step
@@ -563,12 +559,12 @@ __device__ __forceinline__ void ns_finish8(const NsPtrs& p, int it, int mat, int
     }
 }
 
-// f0 .. f2: scale factors of the epilogue (below); low: what is written are pairs (0: the next product takes one plane)
-struct NsScale { float f0, f1, f2; int low, zero_grad; };
+// f0 .. f2: scale factors of the epilogue (below)
+struct NsScale { float f0, f1, f2; int zero_grad; };
 __device__ __forceinline__ float ns_poly(const NsScale& f, float square, float a, bool diagonal) { return fmaf(f.f1, a, f.f0 * square) + (diagonal ? f.f2 : 0.f); }
 
-template <int KIND, int PL, int EPI>
-__global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_HALF && !(EPI == EPI_GRAM && PL == 2) ? 3 : 2) void ns_gemm_kernel(
+template <int KIND, int EPI>
+__global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_HALF && EPI != EPI_GRAM ? 3 : 2) void ns_gemm_kernel(
     const NsTable t, const NsPtrs p, half_t* __restrict__ ws, const float* __restrict__ hyper, int which, const NsScale f) {
     extern __shared__ __attribute__((aligned(512))) unsigned char smem[];
     using Tile = NsTile<KIND>;
@@ -599,16 +595,16 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_HALF && !(E
         constexpr bool LK = decltype(lk)::value, RK = decltype(rk)::value;
         if constexpr (KIND == TILE_32) {
             f32x4 acc[1];
-            ns_product_ksplit<TR, Tile::RING, PL, LK, RK>(L, R, K, smem, acc);
+            ns_product_ksplit<TR, Tile::RING, LK, RK>(L, R, K, smem, acc);
             *reinterpret_cast<f32x4*>(S + ((wave >> 1) * 16 + (lane & 15)) * PITCH + (wave & 1) * 16 + (lane >> 4) * 4) = acc[0];
         } else if constexpr (KIND == TILE_64) {
             f32x4 acc[4];
-            ns_product_ksplit<TR, Tile::RING, PL, LK, RK>(L, R, K, smem, acc);
+            ns_product_ksplit<TR, Tile::RING, LK, RK>(L, R, K, smem, acc);
 #pragma unroll
             for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(S + (wave * 16 + (lane & 15)) * PITCH + j * 16 + (lane >> 4) * 4) = acc[j];
         } else {
-            NsSums<TR / 32, TC / 32, PL, false> acc;
-            ns_product<TR, TC, Tile::RING, PL, LK, RK>(L, R, K, smem, acc);
+            NsSums<TR / 32, TC / 32, false> acc;
+            ns_product<TR, TC, Tile::RING, LK, RK>(L, R, K, smem, acc);
             float* mine = S + ((wave >> 1) * (TR / 2) + (lane & 15)) * PITCH + (wave & 1) * (TC / 2) + (lane >> 4) * 4;
             __syncthreads();                                         // every wave has read its last stage: the ring is free
 #pragma unroll
@@ -650,10 +646,8 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_HALF && !(E
         }
         // GRAM: f0 = sA / sX^2, f2 = -shift sA.  POLY: f0 = c sP / sA^2, f1 = b' sP / sA, f2 = a' sP.  MULT: f0 = sX' / (sP sX).  Last: 1 / (sP sX)
         if constexpr (EPI == EPI_POLY) {
-            const half_t* A = base + off_a(d) + ns_at(PL == 2, r, c, d.mp);
-            const half8 ah = *reinterpret_cast<const half8*>(A);
-            half8 al = {0, 0, 0, 0, 0, 0, 0, 0};
-            if constexpr (PL == 2) al = *reinterpret_cast<const half8*>(A + 32);
+            const half_t* A = base + off_a(d) + ns_at(r, c, d.mp);
+            const half8 ah = *reinterpret_cast<const half8*>(A), al = *reinterpret_cast<const half8*>(A + 32);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = ns_poly(f, v[e], (float)ah[e] + (float)al[e], r == c + e);
         } else {
@@ -670,7 +664,7 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_HALF && !(E
                 *reinterpret_cast<f32x4*>(sp + 4) = f32x4{v[4], v[5], v[6], v[7]};
             }
         }
-        if constexpr (SYM || EPI == EPI_MULT) ns_store8(O, f.low, r, c, ld, v);
+        if constexpr (SYM || EPI == EPI_MULT) ns_store8(O, r, c, ld, v);
         else {
             const int n = r < d.rows ? (d.cols - c < 8 ? d.cols - c : 8) : 0;
             if (n > 0) ns_finish8<EPI>(p, it, mat, r, c, n, lr, keep, f.zero_grad, v);
@@ -686,19 +680,19 @@ __global__ __launch_bounds__(256, KIND == TILE_64 ? 1 : KIND == TILE_HALF && !(E
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = S[(lcol8 * 8 + e) * PITCH + lrow];
-            ns_store8(O, f.low, (long)tj * TC + lrow, ti * TR + lcol8 * 8, ld, v);
+            ns_store8(O, (long)tj * TC + lrow, ti * TR + lcol8 * 8, ld, v);
         }
     }
 }
 
 // Polynomial and P X in one launch for smaller sides up to 192: a workgroup forms the 64 rows of P that its 64 x 64 tile needs by itself.  All of A
-// (147 KB as pairs) is on its way to LDS at once; the band of P never leaves it.  Launches of this size last as long as their latencies
+// (147 KB) is on its way to LDS at once; the band of P never leaves it.  Launches of this size last as long as their latencies
 // (start, first load, store, gap: 4 of 5.5 us), so a third of the launches saved is worth the products done m / 64 times over.
 // Eight waves: 2 x 4 over the band's 64 rows and A's m columns, then 2 x 4 over the 64 x 64 tile.
 constexpr int SMALL_M = 192, SMALL_BYTES = SMALL_M * SMALL_M * 4, SMALL_PITCH = 68;
-template <int MT, int PL>
+template <int MT>
 __device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* X, const NsDims& d, int ti, int tj, const NsScale& poly, unsigned char* smem) {
-    constexpr int SK = PL == 2 ? 32 : 64, KT = MT * 64 / SK, STAGE = MT * 64 * 128, X_STAGE = 64 * 128;      // k of a stage, stages, bytes of A's and X's
+    constexpr int SK = 32, KT = MT * 64 / SK, STAGE = MT * 64 * 128, X_STAGE = 64 * 128;      // k of a stage, stages, bytes of A's and X's
     // X's tile takes the place of the first half of A's stages as soon as they are read, the band of P that of the second half; a 64-wide A leaves
     // them room behind it
     constexpr int HALF = (KT + 1) / 2;
@@ -711,7 +705,7 @@ __device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* 
         const NsOperand op = {A, MT * 64, 0};
         unsigned off[MT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) off[i] = ns_source<64, PL, false>(op, wave * MT + i, lane);
+        for (int i = 0; i < MT; ++i) off[i] = ns_source<64, false>(op, wave * MT + i, lane);
 #pragma unroll
         for (int s = 0; s < KT; ++s)
 #pragma unroll
@@ -719,7 +713,7 @@ __device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* 
     }
     const int wr = (wave >> 2) * 32, wc = (wave & 3) * MT * 16;
     half4 ah[2][MT], al[2][MT];                                       // A's own elements under this wave's part of the band
-    NsSums<2, MT, PL, true> acc;
+    NsSums<2, MT, true> acc;
     acc.clear();
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -728,12 +722,12 @@ __device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* 
     auto place = [&](int r, int c, int q) {                           // 4 elements at row r, column c of a stage: byte offset of plane q
         return r * 128 + (((4 * q + ((c % SK) >> 3)) ^ dma_swz64(r)) << 4) + (c & 7) * 2;
     };
-    const unsigned lane_l = ns_lane<64, PL, false>(smem, band + wr, lane), lane_r = ns_lane<64, PL, false>(smem, wc, lane);
+    const unsigned lane_l = ns_lane<64, false>(smem, band + wr, lane), lane_r = ns_lane<64, false>(smem, wc, lane);
     auto square = [&](int s) {
         const unsigned char* st = smem + s * STAGE;
         NsFrags<2, MT> f;
-        ns_read<64, 2, PL, false>(f.l, lane_l + s * STAGE);
-        ns_read<64, MT, PL, false>(f.r, lane_r + s * STAGE);
+        ns_read<64, 2, false>(f.l, lane_l + s * STAGE);
+        ns_read<64, MT, false>(f.r, lane_r + s * STAGE);
 #pragma unroll
         for (int j = 0; j < MT; ++j)
             if ((wc + j * 16) / SK == s) {                            // uniform
@@ -741,7 +735,7 @@ __device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* 
                 for (int i = 0; i < 2; ++i) {
                     const int rr = band + wr + i * 16 + (lane & 15), c = wc + j * 16 + (lane >> 4) * 4;
                     ah[i][j] = *reinterpret_cast<const half4*>(st + place(rr, c, 0));
-                    if constexpr (PL == 2) al[i][j] = *reinterpret_cast<const half4*>(st + place(rr, c, 1));
+                    al[i][j] = *reinterpret_cast<const half4*>(st + place(rr, c, 1));
                 }
             }
         ns_mfma<false>(f, acc);
@@ -761,9 +755,9 @@ __device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* 
     ns_barrier();
     {
         const NsOperand op = {X, d.cp, (d.tall ? ti : tj) * 64};
-        const half_t* src = d.tall ? ns_base<PL, false>(op) : ns_base<PL, true>(op);
-        const long step = d.tall ? ns_step<PL, false>(op) : ns_step<PL, true>(op);
-        const unsigned off = d.tall ? ns_source<64, PL, false>(op, wave, lane) : ns_source<64, PL, true>(op, wave, lane);
+        const half_t* src = d.tall ? ns_base<false>(op) : ns_base<true>(op);
+        const long step = d.tall ? ns_step<false>(op) : ns_step<true>(op);
+        const unsigned off = d.tall ? ns_source<64, false>(op, wave, lane) : ns_source<64, true>(op, wave, lane);
 #pragma unroll
         for (int s = 0; s < KT; ++s) {
             ns_dma(src, off, lds0 + X_AT + s * X_STAGE + wave * 1024);
@@ -798,21 +792,21 @@ __device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* 
             }
             unsigned char* o = smem + P_AT + (c / SK) * X_STAGE;
             *reinterpret_cast<half4*>(o + place(r, c, 0)) = h;
-            if constexpr (PL == 2) *reinterpret_cast<half4*>(o + place(r, c, 1)) = l;
+            *reinterpret_cast<half4*>(o + place(r, c, 1)) = l;
         }
     ns_wait<0, true>();                                               // X's tile has landed, the band is written
     ns_barrier();
-    NsSums<2, 1, PL, true> out;
+    NsSums<2, 1, true> out;
     out.clear();
     const int o_r = (wave >> 2) * 32, o_c = (wave & 3) * 16;
     auto last = [&](auto tall) {
         constexpr bool TALL = decltype(tall)::value;
-        const unsigned ol = ns_lane<64, PL, false>(smem + (TALL ? X_AT : P_AT), o_r, lane), o_right = ns_lane<64, PL, !TALL>(smem + (TALL ? P_AT : X_AT), o_c, lane);
+        const unsigned ol = ns_lane<64, false>(smem + (TALL ? X_AT : P_AT), o_r, lane), o_right = ns_lane<64, !TALL>(smem + (TALL ? P_AT : X_AT), o_c, lane);
 #pragma unroll
         for (int s = 0; s < KT; ++s) {
             NsFrags<2, 1> f;
-            ns_read<64, 2, PL, false>(f.l, ol + s * X_STAGE);
-            ns_read<64, 1, PL, !TALL>(f.r, o_right + s * X_STAGE);
+            ns_read<64, 2, false>(f.l, ol + s * X_STAGE);
+            ns_read<64, 1, !TALL>(f.r, o_right + s * X_STAGE);
             ns_mfma<false>(f, out);
         }
     };
@@ -825,7 +819,7 @@ __device__ __forceinline__ void ns_small_product(const half_t* A, const half_t* 
     for (int i = 0; i < 2; ++i) *reinterpret_cast<f32x4*>(S + (o_r + i * 16 + (lane & 15)) * SMALL_PITCH + o_c + (lane >> 4) * 4) = out.get(i, 0);
     __syncthreads();
 }
-template <int PL, int EPI>
+template <int EPI>
 __global__ __launch_bounds__(512, 1) void ns_small_kernel(
     const NsTable t, const NsPtrs p, half_t* __restrict__ ws, const float* __restrict__ hyper, int which, const NsScale poly,
     const NsScale f) {
@@ -838,9 +832,9 @@ __global__ __launch_bounds__(512, 1) void ns_small_kernel(
     const int tc = d.cp / 64, ti = tile / tc, tj = tile - ti * tc, tid = threadIdx.x;
     half_t* base = ws + d.ws + mat * d.wsz;
     const half_t *A = base + off_a(d), *X = base + off_x(d, which);
-    if (d.mp == 192) ns_small_product<3, PL>(A, X, d, ti, tj, poly, smem);
-    else if (d.mp == 128) ns_small_product<2, PL>(A, X, d, ti, tj, poly, smem);
-    else ns_small_product<1, PL>(A, X, d, ti, tj, poly, smem);
+    if (d.mp == 192) ns_small_product<3>(A, X, d, ti, tj, poly, smem);
+    else if (d.mp == 128) ns_small_product<2>(A, X, d, ti, tj, poly, smem);
+    else ns_small_product<1>(A, X, d, ti, tj, poly, smem);
     float lr = 0.f, keep = 1.f;
     if constexpr (EPI == EPI_UPDATE) { lr = hyper[0]; keep = 1.f - lr * hyper[2]; lr *= p.scale[it]; }
     const int lrow = tid >> 3, lcol = (tid & 7) * 8, r = ti * 64 + lrow, c = tj * 64 + lcol;
@@ -851,7 +845,7 @@ __global__ __launch_bounds__(512, 1) void ns_small_kernel(
 #pragma unroll
         for (int e = 0; e < 4; ++e) { v[e] = a[e] * f.f0; v[4 + e] = b[e] * f.f0; }
     }
-    if constexpr (EPI == EPI_MULT) ns_store8(base + off_x(d, which ^ 1), f.low, r, c, d.cp, v);
+    if constexpr (EPI == EPI_MULT) ns_store8(base + off_x(d, which ^ 1), r, c, d.cp, v);
     else {
         const int n = r < d.rows ? (d.cols - c < 8 ? d.cols - c : 8) : 0;
         if (n > 0) ns_finish8<EPI>(p, it, mat, r, c, n, lr, keep, f.zero_grad, v);
@@ -946,7 +940,7 @@ double ns_bounds(double bound, double a, double b, double c, double& pmax) {
 // (96 / 144) 251 / 239, 4 x 768^2 (84 / 144) 326 / 354, 12 x 768^2 (252 / 432) 657 / 469, 8 x 384 x 1536 (48 / 288) 277 / 374, 16 x (96 / 576) 493 / 439.
 // 128 x 128 / 128 x 64 for one launch: the four products of twelve 384-wide blocks, Gram 52 / 48, polynomial 27 / 25, P X 63 / 67; 4 x 2048^2, Gram
 // 126 / 121, polynomial 130 / 123, P X 179 / 197; ragged stacks of 192 tiles, P X 15 / 12.
-int tile_kind(const NsTable& t, bool large, bool gram, bool sym, int planes, bool tall) {
+int tile_kind(const NsTable& t, bool large, bool gram, bool sym, bool tall) {
     struct Sum { double n = 0., alone = 0., two = 0., three = 0.; } s64, s128, half;
     double n32 = 0.;
     auto add = [](Sum& s, double n, double stages, double alone, double two, double three) {
@@ -957,7 +951,7 @@ int tile_kind(const NsTable& t, bool large, bool gram, bool sym, int planes, boo
     };
     for (int i = 0; i < t.n; ++i) {
         const NsDims& d = t.d[i];
-        const double stages = (gram ? (d.tall ? d.rp : d.cp) : d.mp) * (planes == 2 ? 1. : 0.5) / 32;
+        const double stages = (gram ? (d.tall ? d.rp : d.cp) : d.mp) / 32;
         const double m3 = d.mp / 32, m6 = d.mp / 64, m12 = d.mp / 128;
         const double a = d.count * (sym ? m6 * (m6 + 1) / 2 : (double)(d.rp / 64) * (d.cp / 64));
         const double b = d.count * (sym ? m12 * (m12 + 1) / 2 : (double)(d.rp / 128) * (d.cp / 128));
@@ -966,47 +960,35 @@ int tile_kind(const NsTable& t, bool large, bool gram, bool sym, int planes, boo
         add(s128, b, stages, 0.85, 1.15, 0.);
         add(half, 2. * b, stages, 0.5, 0.75, 1.1);
     }
-    if (planes == 2 && (n32 <= 512 || (n32 <= 640 && s64.two <= 12. * s64.n))) return TILE_32;
+    if (n32 <= 512 || (n32 <= 640 && s64.two <= 12. * s64.n)) return TILE_32;
     const double t64 = ceil(s64.n / 256) * s64.two / s64.n;
     if (!large) return TILE_64;
     const double t128 = s128.n <= 256 ? s128.alone : ceil(s128.n / 512) * s128.two / s128.n;
-    if (gram && planes == 2 && tall) return (half.n <= 256 ? half.alone : fmax(half.alone, fmax(1., half.n / 512) * half.two / half.n)) < t64 ? TILE_HALF : TILE_64;
+    if (gram && tall) return (half.n <= 256 ? half.alone : fmax(half.alone, fmax(1., half.n / 512) * half.two / half.n)) < t64 ? TILE_HALF : TILE_64;
     const double th = half.n <= 256 ? half.alone : half.n <= 512 ? fmax(half.alone, half.two / half.n) : ceil(half.n / 768) * half.three / half.n;
     return th < t64 && th < t128 ? TILE_HALF : t128 < t64 ? TILE_128 : TILE_64;
 }
-template <int KIND, int PL, int EPI>
+template <int KIND, int EPI>
 int launch_gemm_v(NsTable& t, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& f, hipStream_t s) {
     using Tile = NsTile<KIND>;
     const long grid = ns_grid(t, EPI == EPI_GRAM || EPI == EPI_GRAM_ROWS || EPI == EPI_POLY ? TILES_SYM : TILES_MULT, Tile::TR, Tile::TC);
     S3D_REQUIRE(grid >= 0, "newton_schulz: too many tiles");
-    auto k = ns_gemm_kernel<KIND, PL, EPI>;
+    auto k = ns_gemm_kernel<KIND, EPI>;
     if (Tile::BYTES > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, Tile::BYTES);
     hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(256), Tile::BYTES, s, t, p, ws, hyper, which, f);
-    S3D_CHECK_LAUNCH_V("newton_schulz", KIND * 100 + PL * 10 + EPI);
+    S3D_CHECK_LAUNCH_V("newton_schulz", KIND * 10 + EPI);
     return 0;
 }
-// planes of the operands (2 or 1) as they occur: results in bf16 come from single planes, fp32 results and the parameters' step from pairs
-template <int EPI> constexpr bool ns_pairs() { return EPI != EPI_OUT_BF16; }
-template <int EPI> constexpr bool ns_single() { return EPI != EPI_OUT_F32 && EPI != EPI_UPDATE; }
 template <int EPI>
-int launch_gemm(NsPlan& pl, int planes, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& f, hipStream_t s) {
+int launch_gemm(NsPlan& pl, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& f, hipStream_t s) {
     bool tall = false;
     for (int i = 0; i < pl.t.n; ++i) tall |= pl.t.d[i].tall != 0;
-    const int kind = tile_kind(pl.t, pl.pad == 128, EPI == EPI_GRAM, EPI == EPI_GRAM || EPI == EPI_POLY, planes, tall);
+    const int kind = tile_kind(pl.t, pl.pad == 128, EPI == EPI_GRAM, EPI == EPI_GRAM || EPI == EPI_POLY, tall);
     constexpr int ROWS = EPI == EPI_GRAM ? EPI_GRAM_ROWS : EPI;
-    if constexpr (ns_pairs<EPI>()) {
-        if (planes == 2) {
-            if (kind == TILE_32) return launch_gemm_v<TILE_32, 2, EPI>(pl.t, p, ws, hyper, which, f, s);
-            if (kind == TILE_64) return launch_gemm_v<TILE_64, 2, EPI>(pl.t, p, ws, hyper, which, f, s);
-            if (kind == TILE_128) return launch_gemm_v<TILE_128, 2, ROWS>(pl.t, p, ws, hyper, which, f, s);
-            return tall ? launch_gemm_v<TILE_HALF, 2, EPI>(pl.t, p, ws, hyper, which, f, s) : launch_gemm_v<TILE_HALF, 2, ROWS>(pl.t, p, ws, hyper, which, f, s);
-        }
-    }
-    if constexpr (ns_single<EPI>()) {
-        if (planes == 1) return kind == TILE_64 ? launch_gemm_v<TILE_64, 1, EPI>(pl.t, p, ws, hyper, which, f, s)
-                              : kind == TILE_128 ? launch_gemm_v<TILE_128, 1, EPI>(pl.t, p, ws, hyper, which, f, s) : launch_gemm_v<TILE_HALF, 1, EPI>(pl.t, p, ws, hyper, which, f, s);
-    }
-    S3D_REQUIRE(false, "newton_schulz: no kernel for %d planes", planes);
+    if (kind == TILE_32) return launch_gemm_v<TILE_32, EPI>(pl.t, p, ws, hyper, which, f, s);
+    if (kind == TILE_64) return launch_gemm_v<TILE_64, EPI>(pl.t, p, ws, hyper, which, f, s);
+    if (kind == TILE_128) return launch_gemm_v<TILE_128, ROWS>(pl.t, p, ws, hyper, which, f, s);
+    return tall ? launch_gemm_v<TILE_HALF, EPI>(pl.t, p, ws, hyper, which, f, s) : launch_gemm_v<TILE_HALF, ROWS>(pl.t, p, ws, hyper, which, f, s);
 }
 
 // Polynomial and P X in one launch?  Sides that fit, tiles of P X on the CUs once over.  Whole call, two launches / one, us: 192 x 192 93 / 76, the
@@ -1021,20 +1003,14 @@ bool small_sides(const NsTable& t) {
     return n <= 256;
 }
 template <int EPI>
-int launch_small(NsPlan& pl, int planes, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& poly, const NsScale& mult, hipStream_t s) {
+int launch_small(NsPlan& pl, const NsPtrs& p, half_t* ws, const float* hyper, int which, const NsScale& poly, const NsScale& mult, hipStream_t s) {
     const long grid = ns_grid(pl.t, TILES_MULT);
     S3D_REQUIRE(grid >= 0, "newton_schulz: too many tiles");
-    auto run = [&](auto k) {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_BYTES);
-        hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(512), SMALL_BYTES, s, pl.t, p, ws, hyper, which, poly, mult);
-        S3D_CHECK_LAUNCH_V("newton_schulz_small", planes * 10 + EPI);
-        return 0;
-    };
-    if constexpr (ns_pairs<EPI>())
-        if (planes == 2) return run(ns_small_kernel<2, EPI>);
-    if constexpr (ns_single<EPI>())
-        if (planes == 1) return run(ns_small_kernel<1, EPI>);
-    S3D_REQUIRE(false, "newton_schulz: no kernel for %d planes", planes);
+    auto k = ns_small_kernel<EPI>;
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_BYTES);
+    hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(512), SMALL_BYTES, s, pl.t, p, ws, hyper, which, poly, mult);
+    S3D_CHECK_LAUNCH_V("newton_schulz_small", EPI);
+    return 0;
 }
 
 template <int SRC, int LAST>
@@ -1046,16 +1022,12 @@ int ns_run(NsPlan& pl, const NsPtrs& p, const S3dNsArgs& a, const float* hyper, 
     S3D_REQUIRE(at >= 0, "newton_schulz: too many matrices");
     hipLaunchKernelGGL(ns_sumsq_kernel<SRC>, dim3((unsigned)at), dim3(256), 0, s, t, p, hyper, a.nesterov, part);
     S3D_CHECK_LAUNCH_V("newton_schulz_sumsq", SRC);
-    // Results kept in bf16: the last two steps run on the hi planes alone.  What they round (2^-12, X and P once a step) is multiplied by at most a
-    // per step up to the result: 2 * 2^-12 (a^2 + a) = 0.7 % of its 2-norm at the very most.  Measured beside the 0.17 % of the result's own
-    // rounding: 0.05 - 0.1 % for noise and for a few strong directions, 0.3 % for a matrix of rank one; a third such step would triple it.
-    const int plain_from = LAST == EPI_OUT_BF16 ? a.steps - 2 : a.steps;
     const bool small = small_sides(t);
     double bound = 1.001;
     float sx = pow2_under(32768., bound);
     at = ns_grid(t, TILES_LOAD);
     S3D_REQUIRE(at >= 0, "newton_schulz: too many tiles");
-    hipLaunchKernelGGL(ns_load_kernel<SRC>, dim3((unsigned)at), dim3(256), 0, s, t, p, hyper, a.nesterov, part, a.eps, sx, plain_from > 0, ws);
+    hipLaunchKernelGGL(ns_load_kernel<SRC>, dim3((unsigned)at), dim3(256), 0, s, t, p, hyper, a.nesterov, part, a.eps, sx, ws);
     S3D_CHECK_LAUNCH_V("newton_schulz_load", SRC);
     for (int k = 0; k < a.steps; ++k) {
         double pmax;
@@ -1064,16 +1036,15 @@ int ns_run(NsPlan& pl, const NsPtrs& p, const S3dNsArgs& a, const float* hyper, 
         // singular values are about 1, that square is a tenth of A^2 and so is what its sum loses (the whole result: a third less).
         const double shift = 0.375 * bound * bound, a1 = a.a + (a.b + a.c * shift) * shift, b1 = a.b + 2. * a.c * shift;
         const float sa = pow2_under(32768., bound * bound - shift), sp = pow2_under(32768., pmax), sn = pow2_under(32768., next);
-        const int planes = k >= plain_from ? 1 : 2, low = planes == 2, low_x = k + 1 < plain_from;
-        if (int rc = launch_gemm<EPI_GRAM>(pl, planes, p, ws, hyper, k & 1, {sa / (sx * sx), 0.f, -(float)shift * sa, low, 0}, s)) return rc;
-        const NsScale poly = {a.c * sp / (sa * sa), (float)b1 * sp / sa, (float)a1 * sp, low, 0}, mult = {sn / (sp * sx), 0.f, 0.f, low_x, 0}, last = {1.f / (sp * sx), 0.f, 0.f, 0, a.zero_grad};
+        if (int rc = launch_gemm<EPI_GRAM>(pl, p, ws, hyper, k & 1, {sa / (sx * sx), 0.f, -(float)shift * sa, 0}, s)) return rc;
+        const NsScale poly = {a.c * sp / (sa * sa), (float)b1 * sp / sa, (float)a1 * sp, 0}, mult = {sn / (sp * sx), 0.f, 0.f, 0}, last = {1.f / (sp * sx), 0.f, 0.f, a.zero_grad};
         const bool end = k + 1 == a.steps;
         int rc;
         if (small) {
-            rc = end ? launch_small<LAST>(pl, planes, p, ws, hyper, k & 1, poly, last, s) : launch_small<EPI_MULT>(pl, planes, p, ws, hyper, k & 1, poly, mult, s);
+            rc = end ? launch_small<LAST>(pl, p, ws, hyper, k & 1, poly, last, s) : launch_small<EPI_MULT>(pl, p, ws, hyper, k & 1, poly, mult, s);
         } else {
-            rc = launch_gemm<EPI_POLY>(pl, planes, p, ws, hyper, k & 1, poly, s);
-            if (!rc) rc = end ? launch_gemm<LAST>(pl, planes, p, ws, hyper, k & 1, last, s) : launch_gemm<EPI_MULT>(pl, planes, p, ws, hyper, k & 1, mult, s);
+            rc = launch_gemm<EPI_POLY>(pl, p, ws, hyper, k & 1, poly, s);
+            if (!rc) rc = end ? launch_gemm<LAST>(pl, p, ws, hyper, k & 1, last, s) : launch_gemm<EPI_MULT>(pl, p, ws, hyper, k & 1, mult, s);
         }
         if (rc) return rc;
         sx = sn;
