@@ -386,6 +386,7 @@ class VoxelEngine:
         self.dropout_p = 0.0
         self.dropout_seed = torch.zeros(1, dtype=torch.int64, device=self.device)
         self.muon = None                           # set_muon: matrix parameters by s3d_muon_step, the others by Adam
+        self._muon_since = 0                       # the step count when set_muon took the matrices over
 
     # ------------------------------------------------------------------ parameters
     def _build_param_tables(self):
@@ -466,6 +467,8 @@ class VoxelEngine:
         eps = cur['eps'] if eps is None else eps
         grad_scale = cur['grad_scale'] if grad_scale is None else grad_scale
         cur_step = cur['step'] if step is None else int(step)
+        if getattr(self, 'muon', None) is not None:
+            self._muon_since += cur_step - cur['step']       # the steps taken since set_muon stay the difference
         st = np.zeros(9, dtype=np.int32)
         st[:7] = np.array([lr, betas[0], betas[1], eps, grad_scale, 0.0, 0.0], dtype=np.float32).view(np.int32)
         st[7] = cur_step
@@ -476,7 +479,8 @@ class VoxelEngine:
         """From now on train_step / optimizer_step update the matrix parameters of the transformer (attn.qkv, attn.proj, mlp.fc1, mlp.fc2 weights of
         every block, the four of group_embed) with orthogonalised momentum (s3d_muon_step; the Adam arena m holds the momentum) and everything
         else with Adam as before (set_optimizer).  lr, momentum, weight_decay and grad_scale live on the device, so a captured step follows
-        them; left at None they keep their value (at first 1e-3, 0.95, 0, 1).  The rest is baked into captured graphs.  unset_muon() goes back.
+        them; left at None they keep their value (at first 1e-3, 0.95, 0, 1).  The rest is baked into captured graphs.  unset_muon() goes back
+        to Adam, which begins anew.  The moments of the matrices (arena m, v) that a run with set_muon leaves are for set_muon to go on with, not for Adam.
         Single process: the data-parallel trainers update slices of the arena with Adam and refuse."""
         if not hasattr(self, '_muon_hyper'):
             self._muon_hyper = torch.tensor([1e-3, 0.95, 0.0, 1.0], dtype=torch.float32, device=self.device)
@@ -485,14 +489,24 @@ class VoxelEngine:
                 self._muon_hyper[i:i + 1].fill_(float(v))
         ops.muon_scale(scale, 1, 1)                # (an unknown rule is refused here, not in the middle of a step)
         muon = (bool(nesterov), int(steps), tuple(float(c) for c in coefficients), scale)
+        if self.muon is None:
+            self._muon_since = self.optimizer_state()['step']
         if muon != self.muon:
             self.capture_epoch += 1                # trainers holding their own captures re-capture (and refuse); this engine's cache is keyed by it
         self.muon = muon
 
     def unset_muon(self):
-        if self.muon is not None:
-            self.capture_epoch += 1
+        """Back to Adam for every parameter.  If a step ran meanwhile, Adam begins anew: both moments 0, step count 0, its hyper-parameters kept.  The
+        second moments of the matrices were not kept up, and the one step count behind the bias corrections is all parameters': going on with it would
+        divide the first updates by next to nothing."""
+        if self.muon is None:
+            return
+        self.capture_epoch += 1
         self.muon = None
+        if self.optimizer_state()['step'] != self._muon_since:       # (counted on the device, by replayed steps too)
+            self.arena.m.zero_()
+            self.arena.v.zero_()
+            self.set_optimizer(step=0)
 
     def set_dropout(self, p, seed=None):
         """Dropout of nn.TransformerEncoderLayer inside group_embed (vit_3d_2d_pretrain.py:381; p = 0.1 when model.train()).
