@@ -482,13 +482,18 @@ class VoxelEngine:
         them; left at None they keep their value (at first 1e-3, 0.95, 0, 1).  The rest is baked into captured graphs.  unset_muon() goes back
         to Adam, which begins anew.  The moments of the matrices (arena m, v) that a run with set_muon leaves are for set_muon to go on with, not for Adam.
         Single process: the data-parallel trainers update slices of the arena with Adam and refuse."""
+        # what the step would refuse is refused here, before anything is changed
+        muon = (bool(nesterov), int(steps), tuple(float(c) for c in coefficients), scale)
+        hyper = [None if v is None else float(v) for v in (lr, momentum, weight_decay, grad_scale)]
+        if not abs(ops.muon_scale(scale, 1, 1)) < 3e38:          # (held in fp32)
+            raise ValueError(f'set_muon: non-finite scale {scale}')
         if not hasattr(self, '_muon_hyper'):
             self._muon_hyper = torch.tensor([1e-3, 0.95, 0.0, 1.0], dtype=torch.float32, device=self.device)
-        for i, v in enumerate((lr, momentum, weight_decay, grad_scale)):
+        with torch.cuda.device(self.device):
+            ops.muon_step([], [], [], self._muon_hyper, steps=muon[1], coefficients=muon[2])
+        for i, v in enumerate(hyper):
             if v is not None:
-                self._muon_hyper[i:i + 1].fill_(float(v))
-        ops.muon_scale(scale, 1, 1)                # (an unknown rule is refused here, not in the middle of a step)
-        muon = (bool(nesterov), int(steps), tuple(float(c) for c in coefficients), scale)
+                self._muon_hyper[i:i + 1].fill_(v)
         if self.muon is None:
             self._muon_since = self.optimizer_state()['step']
         if muon != self.muon:
@@ -1001,10 +1006,10 @@ class VoxelEngine:
             raise RuntimeError('muon_step: call set_muon first')
         nesterov, steps, coefficients, scale = self.muon
         a, stacks = self.arena, self.muon_stacks()
-        self.adam_begin()
         stack = lambda t: [t.as_strided((n, r, c), (stride, c, 1), a.offsets[k]) for k, n, r, c, stride in stacks]
         ops.muon_step(stack(a.p), stack(a.g), stack(a.m), self._muon_hyper, planes=list(zip(stack(a.hi), stack(a.lo))), nesterov=nesterov, steps=steps,
                       coefficients=coefficients, scale=scale, zero_grad=zero_grad)
+        self.adam_begin()                          # behind the call that checks its arguments: a refused step is not counted
         self._adam_ranges([(a.offsets[k] + i * stride, r * c) for k, n, r, c, stride in stacks for i in range(n)], zero_grad)
         self._refresh_conv_planes()
 
