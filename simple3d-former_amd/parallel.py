@@ -161,6 +161,12 @@ def graph_collectives_preflight(device_index, group=None, timeout_s=None, sharde
     return ok, detail
 
 
+def _require_adam(engine, who):
+    """The trainers update slices of the arena with Adam: refused before a step begins, not behind its backward and its collectives."""
+    if getattr(engine, 'muon', None) is not None:
+        raise RuntimeError(f'{who}: set_muon is in effect (the data-parallel trainers step with Adam: unset_muon first)')
+
+
 class DataParallelTrainer:
     """Fused training step (forward, loss, backward, all-reduce, Adam) for one rank."""
 
@@ -272,6 +278,7 @@ class DataParallelTrainer:
     # ---- eager step -------------------------------------------------------------------------------------------
     def step_eager(self, x, y, weight=None):
         eng, B = self.eng, x.shape[0]
+        _require_adam(eng, 'DataParallelTrainer')
         eng.advance_dropout_seed()
         loss = eng.forward_loss(x, y, weight)
         with eng.owning_grads():            # this step owns the gradient arena (zeroed by its Adam, one backward): the grouped wgrads may store
@@ -294,6 +301,7 @@ class DataParallelTrainer:
 
     def capture(self, B, weight=None):
         eng = self.eng
+        _require_adam(eng, 'DataParallelTrainer')
         sx = torch.zeros(B, 1, eng.V, eng.V, eng.V, dtype=torch.float32, device=eng.device)
         sy = torch.zeros(B, dtype=torch.int64, device=eng.device)
         state = (eng.arena.p, eng.arena.m, eng.arena.v, eng.arena.g, eng.adam_state, eng.dropout_seed)
@@ -436,7 +444,7 @@ class DataParallelTrainer:
         """Replays the captured step on the static buffers (cap['x'], cap['y'] must already hold the batch)."""
         cap = self._cap
         if cap['epoch'] != self.eng.capture_epoch:
-            raise RuntimeError('the captured step is stale (set_dropout changed a value baked into the graphs): capture() again')
+            raise RuntimeError('the captured step is stale (set_dropout or set_muon changed a value baked into the graphs): capture() again')
         if 'whole' in cap:
             cap['whole'].replay()
             return cap['loss'][0]
@@ -684,6 +692,7 @@ class ShardedDataParallelTrainer:
         return state.get('loss')
 
     def step_eager(self, x, y, weight=None):
+        _require_adam(self.eng, 'ShardedDataParallelTrainer')
         return self._step_body(x, y, weight, lambda i, fn: fn())
 
     def sync_parameters(self):
@@ -707,6 +716,7 @@ class ShardedDataParallelTrainer:
     # ---- HIP-graph step ------------------------------------------------------------------------------------------------------------------
     def capture(self, B, weight=None):
         eng = self.eng
+        _require_adam(eng, 'ShardedDataParallelTrainer')
         sx = torch.zeros(B, 1, eng.V, eng.V, eng.V, dtype=torch.float32, device=eng.device)
         sy = torch.zeros(B, dtype=torch.int64, device=eng.device)
         state = (eng.arena.p, eng.arena.m, eng.arena.v, eng.arena.g, eng.adam_state, eng.dropout_seed)
@@ -761,7 +771,7 @@ class ShardedDataParallelTrainer:
     def step_graph(self):
         cap = self._cap
         if cap['epoch'] != self.eng.capture_epoch:
-            raise RuntimeError('the captured step is stale (set_dropout changed a value baked into the graphs): capture() again')
+            raise RuntimeError('the captured step is stale (set_dropout or set_muon changed a value baked into the graphs): capture() again')
         if 'whole' in cap:
             cap['whole'].replay()
             self.pending = True
