@@ -1120,7 +1120,13 @@ struct NsRanges {
     NsRanges(const NsRanges&) = delete;
     NsRanges& operator=(const NsRanges&) = delete;
     void add(const void* p, int size, long stride, long ld, int count, int rows, int cols, bool write, int item) {
-        v[n++] = MatRange{(uintptr_t)p, size, stride, ld, count, rows, cols, write, item};
+        uintptr_t at = (uintptr_t)p;
+        if (count == 1) stride = 0;                                  // (says nothing)
+        if (stride < 0) {                                            // an input may run backwards: the same matrices from the lowest one up
+            at += (uintptr_t)((count - 1) * stride * size);
+            stride = -stride;
+        }
+        v[n++] = MatRange{at, size, stride, ld, count, rows, cols, write, item};
     }
     // same_item: also tensors of one item
     int check(const char* who, bool same_item) {
@@ -1161,7 +1167,7 @@ int s3d_launch_orthogonalize(const S3dOrthoItem* items, int n, const S3dNsArgs* 
     for (int i = 0; i < n; ++i) {
         const S3dOrthoItem& q = items[i];
         if (q.count == 0 || q.rows == 0 || q.cols == 0) continue;
-        if (q.x_stride >= 0) used.add(q.x, a->x_bf16 ? 2 : 4, q.x_stride, q.x_ld, q.count, q.rows, q.cols, false, i);
+        used.add(q.x, a->x_bf16 ? 2 : 4, q.x_stride, q.x_ld, q.count, q.rows, q.cols, false, i);
         used.add(q.out, a->out_bf16 ? 2 : 4, q.out_stride, q.out_ld, q.count, q.rows, q.cols, true, i);
     }
     if (int rc = used.check(who, false)) return rc;
