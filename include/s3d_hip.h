@@ -256,8 +256,8 @@ int s3d_attention_bwd(const S3dAttnArgs* args, s3d_stream_t stream);
  *   pos             [rows] table row of every token, or NULL: row r takes table row (r / st) % T (st = 1: sequences of T tokens one after the
  *                   other; st = number of sequences: token-major rows).  A position outside [0, T) leaves the token unrotated (class tokens: -1).
  *   *_lo            optional low planes of split-bf16 tensors; the gains may be NULL (= 1).
- * out may be qkv itself (same pointers and pitch; the value heads are then not touched); any other overlap of what is written is refused.  For a
- * backward pass keep the input qkv.
+ * out may be qkv itself (same pointers and pitch; the value heads are then not touched); any other overlap of what is written (the
+ * gains' gradients and partial included) with what is read or written is refused.  For a backward pass keep the input qkv.
  * Backward: dout = gradient of out; dqkv (may be dout itself) = gradient of qkv; dq_gain / dk_gain [hd] are stored, or added to when
  * `accumulate`; they are also computed when the gains are NULL, and may not be one tensor.  partial = scratch of partial_blocks >= s3d_qk_norm_blocks(..) times 2 * hd
  * floats.  No atomics: bitwise reproducible. */

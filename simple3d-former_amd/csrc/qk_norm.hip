@@ -326,6 +326,23 @@ int check(const S3dQkNormArgs& a, bool bwd) {
                 S3D_REQUIRE(!in[k] || (in[k] == out[i] && ldi[k] == ldo && (k & 1) == i) || !ranges_meet(range(out[i], ldo), range(in[k], ldi[k])),
                             "%s: an output plane overlaps an input plane", who);
         S3D_REQUIRE(!out[1] || !ranges_meet(range(out[0], ldo), range(out[1], ldo)), "%s: the output planes overlap", who);
+        // nor may what is written share memory with the gains, tables and positions, nor the gains' gradients and their partial sums with anything
+        auto flat = [](const void* p, size_t n) { return FlatRange{(uintptr_t)p, p ? n * 4 : 0}; };
+        const FlatRange read[5] = {flat(a.q_gain, a.hd), flat(a.k_gain, a.hd), flat(a.cos_t, a.cos_t ? (size_t)a.T * (a.hd / 2) : 0),
+                                   flat(a.sin_t, a.cos_t ? (size_t)a.T * (a.hd / 2) : 0), flat(a.cos_t ? a.pos : nullptr, a.rows)};
+        const size_t sums = bwd ? (size_t)s3d_qk_norm_blocks(a.rows, a.H, a.Hkv, a.hd) * 2 * a.hd : 0;
+        const FlatRange written[3] = {flat(bwd ? a.dq_gain : nullptr, a.hd), flat(bwd ? a.dk_gain : nullptr, a.hd), flat(bwd ? a.partial : nullptr, sums)};
+        for (const FlatRange& f : read) {
+            if (!f.bytes) continue;
+            for (int i = 0; i < 2; ++i) S3D_REQUIRE(!out[i] || !ranges_meet(range(out[i], ldo), f), "%s: an output plane overlaps a gain, a table or the positions", who);
+            for (const FlatRange& w : written) S3D_REQUIRE(!ranges_meet(w, f), "%s: a gain's gradient or partial overlaps a gain, a table or the positions", who);
+        }
+        for (const FlatRange& w : written) {
+            if (!w.bytes) continue;
+            for (int i = 0; i < 2; ++i) S3D_REQUIRE(!out[i] || !ranges_meet(range(out[i], ldo), w), "%s: a gain's gradient or partial overlaps an output plane", who);
+            for (int k = 0; k < 4; ++k) S3D_REQUIRE(!in[k] || !ranges_meet(range(in[k], ldi[k]), w), "%s: a gain's gradient or partial overlaps an input plane", who);
+        }
+        S3D_REQUIRE(!ranges_meet(written[0], written[2]) && !ranges_meet(written[1], written[2]), "%s: partial overlaps a gain's gradient", who);
     }
     return 0;
 }

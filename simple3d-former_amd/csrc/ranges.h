@@ -32,3 +32,13 @@ inline bool ranges_meet(const MatRange& x, const MatRange& y) {
     }
     return true;
 }
+
+struct FlatRange { uintptr_t at; size_t bytes; };
+inline bool ranges_meet(const FlatRange& x, const FlatRange& y) { return x.at < y.at + y.bytes && y.at < x.at + x.bytes; }
+// One matrix and a contiguous piece of memory: exact, what lies between the rows is not the matrix's.
+inline bool ranges_meet(const MatRange& m, const FlatRange& f) {
+    if (f.at + f.bytes <= m.at || f.at >= m.end()) return false;
+    if (f.at < m.at) return true;
+    const size_t pitch = (size_t)m.ld * m.size, off = (f.at - m.at) % pitch;
+    return off < (size_t)m.cols * m.size || off + f.bytes > pitch;
+}
