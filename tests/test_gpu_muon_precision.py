@@ -45,3 +45,24 @@ def test_bf16_results_of_hard_spectra_are_rounded_once(kind):
     x = x.to('cuda:0')
     assert torch.equal(ops.orthogonalize(x, out_dtype=torch.bfloat16), ops.orthogonalize(x).to(torch.bfloat16))
     assert rel(ops.orthogonalize(x, out_dtype=torch.bfloat16), oracle(x)) <= 2.0 ** -9
+
+
+# fp32 results of gradient-like spectra, where all directions grow together and an error keeps its size beside the result.
+#   Random part: every step rounds four tensors to pairs, at most 2^-22 of an entry, 2^-22 / sqrt(12) rms: sqrt(5 * 4) 2^-22 / sqrt(12) = 3.1e-7.
+#   One-sided part: sums that begin at zero every 64 k take six truncated products, at most 2^-24 each, half on average: 1.8e-7 of a product.  It
+#   enters through A with |b + 2 c| = 0.7 and through P X with 1, so 3.1e-7 a step, and is multiplied by p'(1) = a + 3 b + 5 c = -0.72 a step later:
+#   3.1e-7 / sqrt(1 - 0.72^2) = 4.4e-7.
+# In quadrature 5.4e-7; if all of the one-sided part adds to the random one, 7.5e-7: bounded by the next power of two.  A^2 instead of (A - shift)^2 gives
+# 0.6e-6 .. 1.3e-6 here, one running sum instead of the restarted ones 0.6e-6 .. 1.5e-6, both 0.7e-6 .. 2.2e-6 (1 / norm in one part adds 2e-8).
+FP32 = 2.0 ** -20
+
+
+@pytest.mark.parametrize('r,c', [(192, 192), (768, 384), (1536, 384), (192, 768), (384, 1536)])
+@pytest.mark.parametrize('L', [1, 12, 40])
+def test_fp32_results_hold_the_stated_error(L, r, c):
+    x = grads(1, r, c)
+    got = ops.orthogonalize(x.expand(L, r, c).contiguous())
+    want = oracle(x)
+    e = [rel(got[i:i + 1], want) for i in (0, L - 1)]
+    print(f'{L} x {r} x {c}: {max(e):.2e}')
+    assert max(e) <= FP32
