@@ -267,8 +267,8 @@ def _ns_args(steps, coefficients, eps, **kw):
 
 def orthogonalize(x, *, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, out_dtype=None, out=None):
     """Newton-Schulz orthogonalisation of a matrix [r, c] or a stack [L, r, c] (fp32 or bf16): s3d_orthogonalize.  The singular values of
-    x / max(|x|_F, eps) go `steps` times through a s + b s^3 + c s^5, the singular vectors stay.  out_dtype: float32 or bfloat16 (default:
-    x's); out: tensor to write into (may be x)."""
+    x / max(|x|_F, eps) go `steps` times through a s + b s^3 + c s^5, the singular vectors stay.  out_dtype: float32 or bfloat16 (the fp32
+    result rounded once; default: x's); out: tensor to write into (may be x)."""
     who = 'orthogonalize'
     types = (torch.float32, torch.bfloat16)
     _same_device(who, x, out)
@@ -301,7 +301,8 @@ def muon_step(params, grads, momenta, hyper, *, planes=None, nesterov=True, step
               zero_grad=False):
     """One optimizer step with orthogonalised momentum over matrix parameters, in place: s3d_muon_step.  params / grads / momenta: lists of fp32
     [r, c] or [L, r, c] tensors (one entry = one stack of equal matrices); hyper: fp32 device tensor {lr, momentum, decay, grad_scale};
-    planes: list of (hi, lo) bf16 tensors laid out like the parameters, refreshed, or None."""
+    planes: list of (hi, lo) bf16 tensors laid out like the parameters, refreshed, or None.  scale: muon_scale's rule; VoxelEngine.set_muon
+    chooses 'match_rms_adamw', whose updates are 0.2 sqrt(max(rows, cols)) times larger than plain ones ('original' on wide or square matrices)."""
     who = 'muon_step'
     f32 = (torch.float32,)
     if not len(params) == len(grads) == len(momenta) or (planes is not None and len(planes) != len(params)):
