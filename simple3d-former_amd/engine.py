@@ -474,15 +474,18 @@ class VoxelEngine:
         st[7] = cur_step
         self.adam_state.copy_(torch.from_numpy(st))
 
-    def set_muon(self, lr=None, momentum=None, weight_decay=None, grad_scale=None, *, nesterov=True, steps=5, coefficients=ops.NS_COEFFICIENTS,
-                 scale='match_rms_adamw'):
+    def set_muon(self, lr=None, momentum=None, weight_decay=None, grad_scale=None, *, nesterov=None, steps=None, coefficients=None, scale=None):
         """From now on train_step / optimizer_step update the matrix parameters of the transformer (attn.qkv, attn.proj, mlp.fc1, mlp.fc2 weights of
         every block, the four of group_embed) with orthogonalised momentum (s3d_muon_step; the Adam arena m holds the momentum) and everything
         else with Adam as before (set_optimizer).  lr, momentum, weight_decay and grad_scale live on the device, so a captured step follows
-        them; left at None they keep their value (at first 1e-3, 0.95, 0, 1).  The rest is baked into captured graphs.  unset_muon() goes back
-        to Adam, which begins anew.  The moments of the matrices (arena m, v) that a run with set_muon leaves are for set_muon to go on with, not for Adam.
+        them (at first 1e-3, 0.95, 0, 1).  nesterov, steps, coefficients and scale (ops.muon_step) are baked into captured graphs; set_muon begins with True, 5,
+        ops.NS_COEFFICIENTS and 'match_rms_adamw'.  What is left at None keeps its value, so a schedule calls set_muon(lr=..).  unset_muon() goes back to
+        Adam, which begins anew.  The moments of the matrices (arena m, v) that a run with set_muon leaves are for set_muon to go on with, not for Adam.
         Single process: the data-parallel trainers update slices of the arena with Adam and refuse."""
         # what the step would refuse is refused here, before anything is changed
+        given = (nesterov, steps, coefficients, scale)
+        kept = self.muon or (True, 5, ops.NS_COEFFICIENTS, 'match_rms_adamw')
+        nesterov, steps, coefficients, scale = (old if new is None else new for new, old in zip(given, kept))
         muon = (bool(nesterov), int(steps), tuple(float(c) for c in coefficients), scale)
         hyper = [None if v is None else float(v) for v in (lr, momentum, weight_decay, grad_scale)]
         if not abs(ops.muon_scale(scale, 1, 1)) < 3e38:          # (held in fp32)
