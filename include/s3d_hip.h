@@ -256,7 +256,8 @@ int s3d_attention_bwd(const S3dAttnArgs* args, s3d_stream_t stream);
  *   pos             [rows] table row of every token, or NULL: row r takes table row (r / st) % T (st = 1: sequences of T tokens one after the
  *                   other; st = number of sequences: token-major rows).  A position outside [0, T) leaves the token unrotated (class tokens: -1).
  *   *_lo            optional low planes of split-bf16 tensors; the gains may be NULL (= 1).
- *                   Squares are added in fp32: a head whose squares pass 3e38 (entries from 1e18 up) becomes zero; a NaN makes its head NaN.
+ *                   Squares are added in fp32: a head whose squares pass 3e38 (entries from 1e18 up) becomes zero; a NaN makes its head NaN;
+ *                   with eps = 0 a head that is zero or below 1e-19 throughout is not finite.
  * out may be qkv itself (same pointers and pitch; the value heads are then not touched); any other overlap of what is written (the
  * gains' gradients and partial included) with what is read or written is refused.  For a backward pass keep the input qkv.
  * Backward: dout = gradient of out; dqkv (may be dout itself) = gradient of qkv; dq_gain / dk_gain [hd] are stored, or added to when
